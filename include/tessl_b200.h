@@ -392,6 +392,142 @@ TESSL_API int32_t tessl_qwen35_add_rms_norm(TesslRuntime *rt, TesslBuf y, TesslB
                                   uint32_t out_as_bf16, uint32_t rows, uint32_t dim, float eps, char *err,
                                   size_t err_len);
 
+/* ------------------------- between the q/k/v and the output projection --- */
+
+/* What lies between a layer's q/k/v projection and its output projection: rotary
+ * positions, a paged cache of keys and values, and attention over it. The
+ * reference has these as kernels of its Metal tower (its rope, kv_store and
+ * flash_attn families); the entries here are this library's own, in its
+ * conventions: device buffers with capacities, everything that the host can see
+ * checked before any launch, nothing allocated, all of it safe to capture.
+ * What only the device can see (lengths, offsets, page ids) is checked by the
+ * kernels, which leave out what points outside. */
+
+/* Rotary positions: the first `rot_dim` columns of a head are rot_dim / 2 pairs,
+ * pair i turned by position * steps[i] / 2^64 turns and scaled by `factor`; the
+ * columns behind them pass unchanged. Pair i is columns (i, i + rot_dim / 2), or
+ * (2 i, 2 i + 1) when interleaved != 0. `steps` is a device buffer of rot_dim / 2
+ * 64-bit integers: position * step modulo 2^64 is the exact angle of every 32-bit
+ * position. */
+typedef struct TesslRope {
+    TesslBuf steps;
+    uint32_t rot_dim;
+    uint32_t interleaved;
+    float factor;
+} TesslRope;
+
+/* How a context longer than the trained one stretches the frequencies
+ * w_i = theta^(-2 i / rot_dim). LINEAR: all divided by `factor`. NTK: the base
+ * becomes theta * factor^(rot_dim / (rot_dim - 2)). WAVELENGTH: waves longer than
+ * original / low are divided, those shorter than original / high stay, between
+ * them a linear blend in original / wavelength. YARN: pairs that turn at least
+ * `high` times within `original` positions stay, those that turn at most `low`
+ * times are divided, a linear ramp over the pairs' index between them, and the
+ * values are scaled by 0.1 ln(factor) + 1. low / high of 0 mean 1 / 4
+ * (WAVELENGTH) and 1 / 32 (YARN). */
+#define TESSL_ROPE_SCALE_NONE 0u
+#define TESSL_ROPE_SCALE_LINEAR 1u
+#define TESSL_ROPE_SCALE_NTK 2u
+#define TESSL_ROPE_SCALE_WAVELENGTH 3u
+#define TESSL_ROPE_SCALE_YARN 4u
+typedef struct TesslRopeScaling {
+    uint32_t kind;
+    double factor;   /* >= 1 */
+    double original; /* trained context in positions: WAVELENGTH and YARN */
+    double low;
+    double high;
+} TesslRopeScaling;
+
+/* The rot_dim / 2 steps of a base and a scaling (NULL: none) into HOST memory,
+ * and the factor that goes with them. No GPU work. */
+TESSL_API int32_t tessl_rope_steps(uint32_t rot_dim, double theta, const TesslRopeScaling *scaling, uint64_t *steps,
+                                   float *factor, char *err, size_t err_len);
+
+/* out[t, h, :] = x[t, h, :] turned by positions[t] (int32 [tokens]); rows of
+ * n_heads * head_dim values, `x_stride` / `out_stride` elements apart (0 = one
+ * behind the other); x and out f32 or bf16, computed in f32. head_dim even and
+ * <= 256. out may be x itself where type and stride agree. */
+TESSL_API int32_t tessl_rope(TesslRuntime *rt, TesslBuf x, TesslBuf positions, TesslBuf out, const TesslRope *rope,
+                             uint32_t tokens, uint32_t n_heads, uint32_t head_dim, uint32_t x_stride,
+                             uint32_t out_stride, uint32_t x_as_bf16, uint32_t out_as_bf16, char *err, size_t err_len);
+
+/* A cache of keys and values in pages of `page_size` tokens, bf16, both of
+ * [num_pages, page_size, n_kv_heads, head_dim] (TOKEN_MAJOR) or
+ * [num_pages, n_kv_heads, page_size, head_dim] (HEAD_MAJOR). head_dim a multiple
+ * of 8, <= 256; any page_size. */
+#define TESSL_KV_TOKEN_MAJOR 0u
+#define TESSL_KV_HEAD_MAJOR 1u
+typedef struct TesslPagedKv {
+    TesslBuf k;
+    TesslBuf v;
+    uint32_t num_pages;
+    uint32_t page_size;
+    uint32_t n_kv_heads;
+    uint32_t head_dim;
+    uint32_t layout;
+} TesslPagedKv;
+
+/* The sequences of a call. kv_lens int32 [num_seqs]: tokens of each in the cache,
+ * its new ones included. q_starts int32 [num_seqs + 1], ascending: the new tokens
+ * of sequence s are rows q_starts[s] .. q_starts[s + 1] - 1 of the call's tokens;
+ * with a NULL q_starts row s is the one new token of sequence s. New token i of n
+ * stands at position kv_len - n + i. page_table int32 [num_seqs, max_pages]: token
+ * t of a sequence lies in slot t % page_size of page page_table[s][t / page_size].
+ * Rows behind q_starts[num_seqs] belong to no sequence and are left as they are. A
+ * page id outside the cache holds no tokens: nothing is written there, and no row
+ * sees them. Tokens past max_pages * page_size do not exist. */
+typedef struct TesslPagedSeqs {
+    TesslBuf page_table;
+    TesslBuf kv_lens;
+    TesslBuf q_starts;
+    uint32_t num_seqs;
+    uint32_t max_pages;
+} TesslPagedSeqs;
+
+/* Zero-centred RMSNorm of each head of the queries and keys
+ * (tessl_qwen35_rms_norm's formula, weights f32 [head_dim]). */
+typedef struct TesslQkNorm {
+    TesslBuf q_weight;
+    TesslBuf k_weight;
+    float eps;
+} TesslQkNorm;
+
+/* Keys and values of new tokens into the pages of their sequences, and their
+ * queries made ready, in one launch: q and k are normed (`norm`, or NULL), turned
+ * by their positions (`rope`, or NULL), k and v stored in the cache, q in q_out
+ * (bf16 [total_new, n_heads, head_dim]). q [total_new, n_heads * head_dim], k and
+ * v [total_new, n_kv_heads * head_dim], f32 or bf16, rows *_stride elements apart
+ * (0 = one behind the other), so that they may be parts of one fused projection.
+ * n_heads = 0: no queries. A token before position 0 of its sequence (kv_len less
+ * than its new tokens) has no place in the cache; only its query is written. */
+TESSL_API int32_t tessl_kv_append_paged(TesslRuntime *rt, TesslBuf q, TesslBuf k, TesslBuf v, TesslBuf q_out,
+                                        const TesslPagedKv *cache, const TesslPagedSeqs *seqs, const TesslRope *rope,
+                                        const TesslQkNorm *norm, uint32_t total_new, uint32_t n_heads,
+                                        uint32_t q_stride, uint32_t k_stride, uint32_t v_stride, uint32_t in_as_bf16,
+                                        char *err, size_t err_len);
+
+/* Bytes of workspace that tessl_attn_paged wants for a call of these sizes; 0 for
+ * sizes that it refuses. The contents need no preparation and mean nothing
+ * between calls. Calls that may overlap on the GPU (graphs replayed on other
+ * streams) need workspaces of their own. */
+TESSL_API uint64_t tessl_attn_paged_workspace_bytes(TesslRuntime *rt, uint32_t total_new, uint32_t n_heads,
+                                                    const TesslPagedKv *cache, const TesslPagedSeqs *seqs);
+
+/* Attention of the new tokens over their sequences' cache:
+ * out[r, h, :] = sum_j p_j v_j / sum_j p_j, p_j = exp(scale * q[r, h, :] . k_j),
+ * over the tokens j that the row sees: all of its sequence, with causal != 0 those
+ * at its own position and before it, with window > 0 (causal only) those fewer
+ * than `window` positions before it. Head h reads key head
+ * h / (n_heads / n_kv_heads). A row that sees nothing gives zeros. q bf16
+ * [total_new, n_heads, head_dim] with rows q_stride elements apart (0 = one behind
+ * the other, else a multiple of 8), out bf16 [total_new, n_heads, head_dim]: what
+ * the output projection reads. Scores, softmax and sums in f32; the weights p are
+ * rounded to bf16 for the product with v, after the sum over them was taken. */
+TESSL_API int32_t tessl_attn_paged(TesslRuntime *rt, TesslBuf q, const TesslPagedKv *cache, const TesslPagedSeqs *seqs,
+                                   TesslBuf out, TesslBuf workspace, uint32_t total_new, uint32_t n_heads,
+                                   uint32_t q_stride, float scale, uint32_t causal, uint32_t window, char *err,
+                                   size_t err_len);
+
 /* ------------------------------------------------- checkpoint -> bank --- */
 
 /* A safetensors file opened read-only (memory-mapped) with its header parsed

@@ -20,7 +20,8 @@ CSRC = HERE / "csrc"
 LIB = HERE / "_lib" / "libtessl_b200.so"
 STEP_DRIVER = HERE / "_lib" / "tessl_step_driver"
 PY_CALL = HERE / "_lib" / ("_tessl_call" + sysconfig.get_config_var("EXT_SUFFIX"))  # of this interpreter
-SOURCES = ["capi.cu", "nn_q4.cu", "nn_q8.cu", "q4_weight.cu", "prefill_gemm.cu", "peer_gather.cu", "qwen35_norm.cu", "mlx_q4_loader.cu"]
+SOURCES = ["capi.cu", "nn_q4.cu", "nn_q8.cu", "q4_weight.cu", "prefill_gemm.cu", "peer_gather.cu", "qwen35_norm.cu", "mlx_q4_loader.cu",
+           "rope_append.cu", "attn_paged.cu"]
 
 
 def nvcc_path() -> str:

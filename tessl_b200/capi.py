@@ -19,6 +19,8 @@ ABI_VERSION = 1
 TESSL_OK, TESSL_ERR, TESSL_PANIC = 0, 1, 2
 ROW_MAJOR, INTERLEAVED4, B200_STAGED = 0, 1, 2
 GEMM_Q4_MLX_MAX_M = 8
+KV_TOKEN_MAJOR, KV_HEAD_MAJOR = 0, 1
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "wavelength": 3, "yarn": 4}
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libtessl_b200.so"
 CALL_PATH = LIB_PATH.parent / ("_tessl_call" + sysconfig.get_config_var("EXT_SUFFIX"))  # built for this interpreter
@@ -55,6 +57,27 @@ class TensorInfo(C.Structure):
 class PeerGather(C.Structure):
     _fields_ = [("buffers", C.c_void_p * 8), ("flags", C.c_void_p * 8), ("rank", C.c_uint32), ("world", C.c_uint32),
                 ("bytes_per_rank", C.c_uint64)]
+
+
+class Rope(C.Structure):
+    _fields_ = [("steps", Buf), ("rot_dim", C.c_uint32), ("interleaved", C.c_uint32), ("factor", C.c_float)]
+
+
+class RopeScaling(C.Structure):
+    _fields_ = [("kind", C.c_uint32), ("factor", C.c_double), ("original", C.c_double), ("low", C.c_double), ("high", C.c_double)]
+
+
+class PagedKv(C.Structure):
+    _fields_ = [("k", Buf), ("v", Buf), ("num_pages", C.c_uint32), ("page_size", C.c_uint32), ("n_kv_heads", C.c_uint32),
+                ("head_dim", C.c_uint32), ("layout", C.c_uint32)]
+
+
+class PagedSeqs(C.Structure):
+    _fields_ = [("page_table", Buf), ("kv_lens", Buf), ("q_starts", Buf), ("num_seqs", C.c_uint32), ("max_pages", C.c_uint32)]
+
+
+class QkNorm(C.Structure):
+    _fields_ = [("q_weight", Buf), ("k_weight", Buf), ("eps", C.c_float)]
 
 
 _ERR = [C.c_char_p, C.c_size_t]
@@ -117,6 +140,13 @@ SIGNATURES = {
     "tessl_qwen35_rms_norm": (C.c_int32, [_RT, Buf, Buf, Buf, _u32, _u32, _u32, C.c_float] + _ERR),
     "tessl_qwen35_residual_add": (C.c_int32, [_RT, Buf, Buf, _u32, _u32] + _ERR),
     "tessl_qwen35_add_rms_norm": (C.c_int32, [_RT, Buf, Buf, Buf, Buf, _u32, _u32, _u32, C.c_float] + _ERR),
+    "tessl_rope_steps": (C.c_int32, [_u32, C.c_double, C.POINTER(RopeScaling), C.POINTER(C.c_uint64), C.POINTER(C.c_float)] + _ERR),
+    "tessl_rope": (C.c_int32, [_RT, Buf, Buf, Buf, C.POINTER(Rope)] + [_u32] * 7 + _ERR),
+    "tessl_kv_append_paged": (C.c_int32, [_RT, Buf, Buf, Buf, Buf, C.POINTER(PagedKv), C.POINTER(PagedSeqs), C.POINTER(Rope),
+                                          C.POINTER(QkNorm)] + [_u32] * 6 + _ERR),
+    "tessl_attn_paged_workspace_bytes": (C.c_uint64, [_RT, _u32, _u32, C.POINTER(PagedKv), C.POINTER(PagedSeqs)]),
+    "tessl_attn_paged": (C.c_int32, [_RT, Buf, C.POINTER(PagedKv), C.POINTER(PagedSeqs), Buf, Buf, _u32, _u32, _u32, C.c_float, _u32,
+                                     _u32] + _ERR),
     "tessl_checkpoint_open": (C.c_void_p, [C.c_char_p] + _ERR),
     "tessl_checkpoint_close": (None, [C.c_void_p]),
     "tessl_checkpoint_tensor_count": (C.c_int32, [C.c_void_p, C.POINTER(C.c_uint64)] + _ERR),
@@ -170,6 +200,7 @@ ERR_LEN = 1024
 NATIVE_OPERATORS = ("gemv_q4_mlx_simd", "gemv_q4_mlx_gate_up_silu", "gemv_q4_mlx_kv", "gemv_q4_mlx_qkv", "swiglu", "gemm_q4_mlx",
                     "gemm_q4_mlx_tensorops", "gemv_q8", "gemm_q8_mlx", "embed_lookup_q4_mlx", "qwen35_rms_norm",
                     "qwen35_residual_add", "qwen35_add_rms_norm")
+NATIVE_ATTENTION = ("rope", "kv_append_paged", "attn_paged")
 
 _fn_cache: dict = {}
 _err_local = threading.local()

@@ -626,6 +626,61 @@ int32_t tessl_qwen35_add_rms_norm(TesslRuntime *rt, TesslBuf y, TesslBuf resid, 
     });
 }
 
+int32_t tessl_rope_steps(uint32_t rot_dim, double theta, const TesslRopeScaling *scaling, uint64_t *steps, float *factor,
+                         char *err, size_t err_len)
+{
+    try {
+        const Result r = tessl::nn::rope_steps(rot_dim, theta, scaling, steps, factor);
+        if (r.empty()) return TESSL_OK;
+        write_err(err, err_len, r);
+        return TESSL_ERR;
+    } catch (...) {
+        write_err(err, err_len, "panic in tessl: rope_steps");
+        return TESSL_PANIC;
+    }
+}
+
+int32_t tessl_rope(TesslRuntime *rt, TesslBuf x, TesslBuf positions, TesslBuf out, const TesslRope *rope, uint32_t tokens,
+                   uint32_t n_heads, uint32_t head_dim, uint32_t x_stride, uint32_t out_stride, uint32_t x_as_bf16,
+                   uint32_t out_as_bf16, char *err, size_t err_len)
+{
+    return guarded(rt, err, err_len, true, [&]() -> Result {
+        if (!rope) return "rope: null rope";
+        return tessl::nn::rope(rt, x, positions, out, *rope, tokens, n_heads, head_dim, x_stride, out_stride, x_as_bf16 != 0,
+                               out_as_bf16 != 0);
+    });
+}
+
+int32_t tessl_kv_append_paged(TesslRuntime *rt, TesslBuf q, TesslBuf k, TesslBuf v, TesslBuf q_out, const TesslPagedKv *cache,
+                              const TesslPagedSeqs *seqs, const TesslRope *rope, const TesslQkNorm *norm, uint32_t total_new,
+                              uint32_t n_heads, uint32_t q_stride, uint32_t k_stride, uint32_t v_stride, uint32_t in_as_bf16,
+                              char *err, size_t err_len)
+{
+    return guarded(rt, err, err_len, true, [&]() -> Result {
+        if (!cache || !seqs) return "kv_append_paged: null descriptor";
+        return tessl::nn::kv_append_paged(rt, q, k, v, q_out, *cache, *seqs, rope, norm, total_new, n_heads, q_stride, k_stride,
+                                          v_stride, in_as_bf16 != 0);
+    });
+}
+
+uint64_t tessl_attn_paged_workspace_bytes(TesslRuntime *rt, uint32_t total_new, uint32_t n_heads, const TesslPagedKv *cache,
+                                          const TesslPagedSeqs *seqs)
+{
+    if (!rt || !cache || !seqs) return 0;
+    return tessl::nn::attn_paged_workspace_bytes(rt, total_new, n_heads, *cache, *seqs);
+}
+
+int32_t tessl_attn_paged(TesslRuntime *rt, TesslBuf q, const TesslPagedKv *cache, const TesslPagedSeqs *seqs, TesslBuf out,
+                         TesslBuf workspace, uint32_t total_new, uint32_t n_heads, uint32_t q_stride, float scale,
+                         uint32_t causal, uint32_t window, char *err, size_t err_len)
+{
+    return guarded(rt, err, err_len, true, [&]() -> Result {
+        if (!cache || !seqs) return "attn_paged: null descriptor";
+        return tessl::nn::attn_paged(rt, q, *cache, *seqs, out, workspace, total_new, n_heads, q_stride, scale, causal != 0,
+                                     window);
+    });
+}
+
 int32_t tessl_q4_mlx_unpack(TesslRuntime *rt, TesslQ4MlxBank bank, TesslQuantShape shape, TesslBuf out_u8, char *err,
                             size_t err_len)
 {

@@ -9,6 +9,8 @@
 #include "../../include/tessl_b200.h"
 
 static PyObject *s_handle, *s_value, *s_ptr, *s_nbytes, *s_packed, *s_sb, *s_rows, *s_cols, *s_group, *s_q, *s_k, *s_v;
+static PyObject *s_steps, *s_rot, *s_inter, *s_factor, *s_ck, *s_cv, *s_pages, *s_psize, *s_nkv, *s_hdim, *s_layout, *s_table, *s_lens,
+    *s_starts, *s_nseqs, *s_maxp, *s_qw, *s_kw, *s_eps;
 static PyObject *error_class; /* TesslError(status, message) */
 
 /* Readers: 1 if the object was understood. An int is taken modulo 2^32 or 2^64, as a ctypes integer argument is. */
@@ -86,6 +88,56 @@ static int as_opt(PyObject *o, TesslBuf *store, const TesslBuf **out)
     if (o == Py_None) return 1;
     *out = store;
     return as_buf(o, store);
+}
+static int attr_f32(PyObject *o, PyObject *name, float *out)
+{
+    PyObject *v = PyObject_GetAttr(o, name);
+    if (!v) return 0;
+    const int ok = as_f32(v, out);
+    Py_DECREF(v);
+    return ok;
+}
+static int attr_flag(PyObject *o, PyObject *name, uint32_t *out)
+{
+    PyObject *v = PyObject_GetAttr(o, name);
+    if (!v) return 0;
+    const int ok = as_flag(v, out);
+    Py_DECREF(v);
+    return ok;
+}
+/* A buffer, or an empty one for None. */
+static int as_buf_or_none(PyObject *o, TesslBuf *out)
+{
+    out->ptr = NULL, out->nbytes = 0;
+    return o == Py_None || as_buf(o, out);
+}
+static int attr_buf_or_none(PyObject *o, PyObject *name, TesslBuf *out)
+{
+    PyObject *v = PyObject_GetAttr(o, name);
+    if (!v) return 0;
+    const int ok = as_buf_or_none(v, out);
+    Py_DECREF(v);
+    return ok;
+}
+static int as_rope(PyObject *o, TesslRope *out)
+{
+    return attr_buf(o, s_steps, &out->steps) && attr_u32(o, s_rot, &out->rot_dim) && attr_flag(o, s_inter, &out->interleaved) &&
+           attr_f32(o, s_factor, &out->factor);
+}
+static int as_norm(PyObject *o, TesslQkNorm *out)
+{
+    return attr_buf(o, s_qw, &out->q_weight) && attr_buf(o, s_kw, &out->k_weight) && attr_f32(o, s_eps, &out->eps);
+}
+static int as_cache(PyObject *o, TesslPagedKv *out)
+{
+    return attr_buf(o, s_ck, &out->k) && attr_buf(o, s_cv, &out->v) && attr_u32(o, s_pages, &out->num_pages) &&
+           attr_u32(o, s_psize, &out->page_size) && attr_u32(o, s_nkv, &out->n_kv_heads) && attr_u32(o, s_hdim, &out->head_dim) &&
+           attr_u32(o, s_layout, &out->layout);
+}
+static int as_seqs(PyObject *o, TesslPagedSeqs *out)
+{
+    return attr_buf(o, s_table, &out->page_table) && attr_buf(o, s_lens, &out->kv_lens) && attr_buf_or_none(o, s_starts, &out->q_starts) &&
+           attr_u32(o, s_nseqs, &out->num_seqs) && attr_u32(o, s_maxp, &out->max_pages);
 }
 /* The runtime's handle, a c_void_p (None once it is closed). */
 static int as_rt(PyObject *o, TesslRuntime **out)
@@ -273,6 +325,47 @@ OP(qwen35_add_rms_norm) /* rt, y, resid, w, out, bf16, rows, dim, eps */
     RUN(tessl_qwen35_add_rms_norm(rt, y, r, w, o, bf16, rows, dim, eps, err, sizeof err));
 }
 
+OP(rope) /* rt, x, positions, out, rope, tokens, heads, head_dim, x_bf16, out_bf16, x_stride, out_stride */
+{
+    TesslRuntime *rt;
+    TesslBuf x, pos, out;
+    TesslRope r;
+    uint32_t tokens, heads, dim, xb, ob, xs, os;
+    NEED(12, as_rt(a[0], &rt) && as_buf(a[1], &x) && as_buf(a[2], &pos) && as_buf(a[3], &out) && as_rope(a[4], &r) &&
+                 as_u32(a[5], &tokens) && as_u32(a[6], &heads) && as_u32(a[7], &dim) && as_flag(a[8], &xb) && as_flag(a[9], &ob) &&
+                 as_u32(a[10], &xs) && as_u32(a[11], &os));
+    RUN(tessl_rope(rt, x, pos, out, &r, tokens, heads, dim, xs, os, xb, ob, err, sizeof err));
+}
+OP(kv_append_paged) /* rt, q, k, v, q_out, cache, seqs, rope, norm, total_new, heads, q_stride, k_stride, v_stride, bf16 */
+{
+    TesslRuntime *rt;
+    TesslBuf q, k, v, qo;
+    TesslPagedKv c;
+    TesslPagedSeqs s;
+    TesslRope r;
+    TesslQkNorm w;
+    uint32_t total, heads, qs, ks, vs, bf16;
+    NEED(15, as_rt(a[0], &rt) && as_buf_or_none(a[1], &q) && as_buf(a[2], &k) && as_buf(a[3], &v) && as_buf_or_none(a[4], &qo) &&
+                 as_cache(a[5], &c) && as_seqs(a[6], &s) && (a[7] == Py_None || as_rope(a[7], &r)) && (a[8] == Py_None || as_norm(a[8], &w)) &&
+                 as_u32(a[9], &total) && as_u32(a[10], &heads) && as_u32(a[11], &qs) && as_u32(a[12], &ks) && as_u32(a[13], &vs) &&
+                 as_flag(a[14], &bf16));
+    RUN(tessl_kv_append_paged(rt, q, k, v, qo, &c, &s, a[7] == Py_None ? NULL : &r, a[8] == Py_None ? NULL : &w, total, heads, qs, ks, vs,
+                              bf16, err, sizeof err));
+}
+OP(attn_paged) /* rt, q, cache, seqs, out, workspace, total_new, heads, scale, causal, window, q_stride */
+{
+    TesslRuntime *rt;
+    TesslBuf q, out, work;
+    TesslPagedKv c;
+    TesslPagedSeqs s;
+    uint32_t total, heads, causal, window, qs;
+    float scale;
+    NEED(12, as_rt(a[0], &rt) && as_buf(a[1], &q) && as_cache(a[2], &c) && as_seqs(a[3], &s) && as_buf(a[4], &out) && as_buf(a[5], &work) &&
+                 as_u32(a[6], &total) && as_u32(a[7], &heads) && as_f32(a[8], &scale) && as_flag(a[9], &causal) && as_u32(a[10], &window) &&
+                 as_u32(a[11], &qs));
+    RUN(tessl_attn_paged(rt, q, &c, &s, out, work, total, heads, qs, scale, causal, window, err, sizeof err));
+}
+
 static PyObject *set_error(PyObject *self, PyObject *cls)
 {
     Py_XSETREF(error_class, Py_NewRef(cls));
@@ -284,6 +377,7 @@ static PyMethodDef methods[] = {
     ENTRY(gemv_q4_mlx_simd), ENTRY(gemv_q4_mlx_gate_up_silu), ENTRY(gemv_q4_mlx_kv), ENTRY(gemv_q4_mlx_qkv), ENTRY(swiglu),
     ENTRY(gemm_q4_mlx), ENTRY(gemm_q4_mlx_tensorops), ENTRY(gemv_q8), ENTRY(gemm_q8_mlx), ENTRY(embed_lookup_q4_mlx),
     ENTRY(qwen35_rms_norm), ENTRY(qwen35_residual_add), ENTRY(qwen35_add_rms_norm),
+    ENTRY(rope), ENTRY(kv_append_paged), ENTRY(attn_paged),
     {"set_error", set_error, METH_O, "The class to raise refusals as: called with (status, message)."},
     {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tessl_call", NULL, -1, methods, NULL, NULL, NULL, NULL};
@@ -295,7 +389,11 @@ PyMODINIT_FUNC PyInit__tessl_call(void)
         const char *name;
     } names[] = {{&s_handle, "handle"}, {&s_value, "value"}, {&s_ptr, "ptr"}, {&s_nbytes, "nbytes"}, {&s_packed, "packed"},
                  {&s_sb, "scales_biases"}, {&s_rows, "rows"}, {&s_cols, "cols"}, {&s_group, "group_size"}, {&s_q, "q_out"},
-                 {&s_k, "k_out"}, {&s_v, "v_out"}};
+                 {&s_k, "k_out"}, {&s_v, "v_out"}, {&s_steps, "steps"}, {&s_rot, "rot_dim"}, {&s_inter, "interleaved"},
+                 {&s_factor, "factor"}, {&s_ck, "k"}, {&s_cv, "v"}, {&s_pages, "num_pages"}, {&s_psize, "page_size"},
+                 {&s_nkv, "n_kv_heads"}, {&s_hdim, "head_dim"}, {&s_layout, "layout"}, {&s_table, "page_table"}, {&s_lens, "kv_lens"},
+                 {&s_starts, "q_starts"}, {&s_nseqs, "num_seqs"}, {&s_maxp, "max_pages"}, {&s_qw, "q_weight"}, {&s_kw, "k_weight"},
+                 {&s_eps, "eps"}};
     for (size_t i = 0; i < sizeof names / sizeof names[0]; ++i)
         if (!(*names[i].at = PyUnicode_InternFromString(names[i].name))) return NULL;
     error_class = Py_NewRef(PyExc_RuntimeError);

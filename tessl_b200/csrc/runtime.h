@@ -351,6 +351,19 @@ Result qwen35_add_rms_norm(TesslRuntime *rt, const TesslBuf &y, const TesslBuf &
                            bool out_as_bf16, uint32_t rows, uint32_t dim, float eps);
 Result embed_lookup_q4_mlx(TesslRuntime *rt, const TesslQ4MlxBank &bank, const TesslBuf &token_ids, const TesslBuf &out,
                            uint32_t vocab, uint32_t hidden, uint32_t group_size, uint32_t n_tokens);
+Result rope_steps(uint32_t rot_dim, double theta, const TesslRopeScaling *scaling, uint64_t *steps, float *factor);
+Result rope(TesslRuntime *rt, const TesslBuf &x, const TesslBuf &positions, const TesslBuf &out, const TesslRope &rope,
+            uint32_t tokens, uint32_t n_heads, uint32_t head_dim, uint32_t x_stride, uint32_t out_stride, bool x_as_bf16,
+            bool out_as_bf16);
+Result kv_append_paged(TesslRuntime *rt, const TesslBuf &q, const TesslBuf &k, const TesslBuf &v, const TesslBuf &q_out,
+                       const TesslPagedKv &cache, const TesslPagedSeqs &seqs, const TesslRope *rope, const TesslQkNorm *norm,
+                       uint32_t total_new, uint32_t n_heads, uint32_t q_stride, uint32_t k_stride, uint32_t v_stride,
+                       bool in_as_bf16);
+uint64_t attn_paged_workspace_bytes(TesslRuntime *rt, uint32_t total_new, uint32_t n_heads, const TesslPagedKv &cache,
+                                    const TesslPagedSeqs &seqs);
+Result attn_paged(TesslRuntime *rt, const TesslBuf &q, const TesslPagedKv &cache, const TesslPagedSeqs &seqs, const TesslBuf &out,
+                  const TesslBuf &workspace, uint32_t total_new, uint32_t n_heads, uint32_t q_stride, float scale, bool causal,
+                  uint32_t window);
 uint64_t q4_mlx_staged_bytes(uint32_t rows, uint32_t cols, uint32_t group_size);
 Result q4_mlx_repack_staged(TesslRuntime *rt, const TesslQ4MlxBank &bank, const TesslQuantShape &shape, const TesslBuf &out);
 Result q4_mlx_unpack(TesslRuntime *rt, const TesslQ4MlxBank &bank, const TesslQuantShape &shape, const TesslBuf &out);

@@ -24,6 +24,8 @@ B200_STAGED = capi.B200_STAGED
 INTERLEAVED4 = capi.INTERLEAVED4
 GEMM_Q4_MLX_MAX_M = capi.GEMM_Q4_MLX_MAX_M
 GEMM_Q4_MLX_TENSOROPS_GROUP_SIZES = (32, 64, 128)
+KV_TOKEN_MAJOR = capi.KV_TOKEN_MAJOR
+KV_HEAD_MAJOR = capi.KV_HEAD_MAJOR
 
 
 @dataclass(frozen=True)
@@ -122,6 +124,70 @@ class QkvOutputs:
 
     def c(self) -> _CQkv:
         return _CQkv(self.q_out.c(), self.k_out.c(), self.v_out.c())
+
+
+@dataclass(frozen=True)
+class RopeScaling:
+    """How a longer context stretches the rotary frequencies (`TesslRopeScaling` in include/tessl_b200.h): `kind` is "linear",
+    "ntk", "wavelength" or "yarn"."""
+    kind: str
+    factor: float
+    original: float = 0.0
+    low: float = 0.0
+    high: float = 0.0
+
+
+@dataclass
+class Rope:
+    """Rotary positions of a head's first `rot_dim` columns (`TesslRope`): built once by `rope_plan`."""
+    steps: GpuBuffer
+    rot_dim: int
+    interleaved: bool
+    factor: float
+
+    def c(self):
+        return capi.Rope(self.steps.c(), self.rot_dim, int(self.interleaved), self.factor)
+
+
+@dataclass
+class PagedKv:
+    """A cache of keys and values in pages, bf16 (`TesslPagedKv`)."""
+    k: GpuBuffer
+    v: GpuBuffer
+    num_pages: int
+    page_size: int
+    n_kv_heads: int
+    head_dim: int
+    layout: int = KV_TOKEN_MAJOR
+
+    def c(self):
+        return capi.PagedKv(self.k.c(), self.v.c(), self.num_pages, self.page_size, self.n_kv_heads, self.head_dim, self.layout)
+
+
+@dataclass
+class PagedSeqs:
+    """The sequences of a call (`TesslPagedSeqs`): page table int32 [num_seqs, max_pages], lengths int32 [num_seqs] with the new
+    tokens counted, first rows int32 [num_seqs + 1] of their new tokens, or None where each has one."""
+    page_table: GpuBuffer
+    kv_lens: GpuBuffer
+    q_starts: Optional[GpuBuffer]
+    num_seqs: int
+    max_pages: int
+
+    def c(self):
+        starts = Buf() if self.q_starts is None else self.q_starts.c()
+        return capi.PagedSeqs(self.page_table.c(), self.kv_lens.c(), starts, self.num_seqs, self.max_pages)
+
+
+@dataclass
+class QkNorm:
+    """Zero-centred RMSNorm of each head of queries and keys (`TesslQkNorm`): weights f32 [head_dim]."""
+    q_weight: GpuBuffer
+    k_weight: GpuBuffer
+    eps: float
+
+    def c(self):
+        return capi.QkNorm(self.q_weight.c(), self.k_weight.c(), self.eps)
 
 
 class Runtime:
@@ -226,7 +292,7 @@ class _Native:
 
     def __getattr__(self, name):
         mod = capi.native()
-        for op in capi.NATIVE_OPERATORS:
+        for op in capi.NATIVE_OPERATORS + capi.NATIVE_ATTENTION:
             setattr(self, op, getattr(mod, op) if mod else lambda *args: False)
         return getattr(self, name)
 
@@ -387,6 +453,61 @@ def qwen35_add_rms_norm(rt: Runtime, y: GpuBuffer, resid: GpuBuffer, w: GpuBuffe
     if _native.qwen35_add_rms_norm(rt, y, resid, w, out, out_as_bf16, rows, dim, eps):
         return
     capi.call("tessl_qwen35_add_rms_norm", rt.handle, y.c(), resid.c(), w.c(), out.c(), int(out_as_bf16), rows, dim, eps)
+
+
+def rope_steps(rot_dim: int, theta: float, scaling: Optional[RopeScaling] = None) -> tuple:
+    """(steps uint64 [rot_dim / 2], factor) of `tessl_rope_steps`: the turn of one position of each pair, as a fraction of 2^64.
+    Host only."""
+    steps, factor = np.zeros(rot_dim // 2, np.uint64), C.c_float(1.0)
+    s = None
+    if scaling is not None:
+        if scaling.kind not in capi.ROPE_SCALINGS:
+            raise ValueError(f"unknown rope scaling {scaling.kind!r}: one of {', '.join(capi.ROPE_SCALINGS)}")
+        s = C.byref(capi.RopeScaling(capi.ROPE_SCALINGS[scaling.kind], scaling.factor, scaling.original, scaling.low, scaling.high))
+    capi.call("tessl_rope_steps", rot_dim, theta, s, steps.ctypes.data_as(C.POINTER(C.c_uint64)), C.byref(factor))
+    return steps, factor.value
+
+
+def rope_plan(rt: Runtime, rot_dim: int, theta: float, *, interleaved: bool = False,
+              scaling: Optional[RopeScaling] = None) -> Rope:
+    """The rotation that a model's layers share, with its steps on the device."""
+    steps, factor = rope_steps(rot_dim, theta, scaling)
+    return Rope(rt.buffer_from(steps), rot_dim, interleaved, factor)
+
+
+def rope(rt: Runtime, x: GpuBuffer, positions: GpuBuffer, out: GpuBuffer, rope: Rope, tokens: int, n_heads: int, head_dim: int,
+         x_as_bf16: bool, out_as_bf16: bool, x_stride: int = 0, out_stride: int = 0) -> None:
+    """Rows of heads turned by their positions (int32 [tokens]); see `tessl_rope` in include/tessl_b200.h."""
+    if _native.rope(rt, x, positions, out, rope, tokens, n_heads, head_dim, x_as_bf16, out_as_bf16, x_stride, out_stride):
+        return
+    capi.call("tessl_rope", rt.handle, x.c(), positions.c(), out.c(), C.byref(rope.c()), tokens, n_heads, head_dim, x_stride, out_stride,
+              int(x_as_bf16), int(out_as_bf16))
+
+
+def kv_append_paged(rt: Runtime, q: Optional[GpuBuffer], k: GpuBuffer, v: GpuBuffer, q_out: Optional[GpuBuffer], cache: PagedKv,
+                    seqs: PagedSeqs, rope: Optional[Rope], norm: Optional[QkNorm], total_new: int, n_heads: int, q_stride: int = 0,
+                    k_stride: int = 0, v_stride: int = 0, in_as_bf16: bool = False) -> None:
+    """New keys and values into the pages of their sequences, normed and rotated on the way, the queries beside them into q_out
+    (bf16); see `tessl_kv_append_paged` in include/tessl_b200.h."""
+    if _native.kv_append_paged(rt, q, k, v, q_out, cache, seqs, rope, norm, total_new, n_heads, q_stride, k_stride, v_stride, in_as_bf16):
+        return
+    capi.call("tessl_kv_append_paged", rt.handle, Buf() if q is None else q.c(), k.c(), v.c(), Buf() if q_out is None else q_out.c(),
+              C.byref(cache.c()), C.byref(seqs.c()), None if rope is None else C.byref(rope.c()),
+              None if norm is None else C.byref(norm.c()), total_new, n_heads, q_stride, k_stride, v_stride, int(in_as_bf16))
+
+
+def attn_paged_workspace_bytes(rt: Runtime, total_new: int, n_heads: int, cache: PagedKv, seqs: PagedSeqs) -> int:
+    """Bytes of workspace that `attn_paged` wants for a call of these sizes; 0 for sizes that it refuses."""
+    return int(capi.load().tessl_attn_paged_workspace_bytes(rt.handle, total_new, n_heads, C.byref(cache.c()), C.byref(seqs.c())))
+
+
+def attn_paged(rt: Runtime, q: GpuBuffer, cache: PagedKv, seqs: PagedSeqs, out: GpuBuffer, workspace: GpuBuffer, total_new: int,
+               n_heads: int, scale: float, causal: bool = True, window: int = 0, q_stride: int = 0) -> None:
+    """Attention of the new tokens over their sequences' cache; see `tessl_attn_paged` in include/tessl_b200.h."""
+    if _native.attn_paged(rt, q, cache, seqs, out, workspace, total_new, n_heads, scale, causal, window, q_stride):
+        return
+    capi.call("tessl_attn_paged", rt.handle, q.c(), C.byref(cache.c()), C.byref(seqs.c()), out.c(), workspace.c(), total_new, n_heads,
+              q_stride, scale, int(causal), window)
 
 
 def q4_mlx_unpack(rt: Runtime, bank: Q4MlxBank, shape: QuantShape, out_u8: GpuBuffer) -> None:
