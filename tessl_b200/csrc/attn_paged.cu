@@ -1,7 +1,11 @@
 // Attention over a paged cache: checks, routes and launches.
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "attn_paged_split.cuh"
+#include "attn_paged_tile.cuh"
+#include "tensormap.h"
 
 namespace tessl {
 namespace {
@@ -10,20 +14,35 @@ using attn::Params;
 
 uint32_t padded_dim(uint32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : d <= 192 ? 192 : 256; }
 
-template <int DP>
-size_t split_workspace(const TesslRuntime *rt)
-{
-    return (size_t)rt->sm_count * 2 * attn::Part<attn::kSplitRows, DP>::FLOATS * sizeof(float);
-}
-
-size_t workspace_of(const TesslRuntime *rt, uint32_t head_dim)
+/// f(std::integral_constant<int, DP>) for the padded width of a head.
+template <typename F>
+auto with_dim(uint32_t head_dim, F f)
 {
     switch (padded_dim(head_dim)) {
-    case 64: return split_workspace<64>(rt);
-    case 128: return split_workspace<128>(rt);
-    case 192: return split_workspace<192>(rt);
-    default: return split_workspace<256>(rt);
+    case 64: return f(std::integral_constant<int, 64>{});
+    case 128: return f(std::integral_constant<int, 128>{});
+    case 192: return f(std::integral_constant<int, 192>{});
+    default: return f(std::integral_constant<int, 256>{});
     }
+}
+
+/// Tokens per TMA box: a power of two that divides a page; fewer than eight would break the swizzle's groups of eight rows.
+uint32_t box_of(uint32_t page_size) { return std::min(page_size & (0u - page_size), attn::kTileKeys); }
+
+/// Whether a call of these sizes goes to the tensor-core tiles: enough rows for each key head of a sequence to fill some of a tile.
+bool wants_tiles(const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t group)
+{
+    return seqs.q_starts.ptr && cache.num_pages > 0 && box_of(cache.page_size) >= 8 && elems(total_new, group) > 32ull * seqs.num_seqs;
+}
+
+uint64_t workspace_of(const TesslRuntime *rt, const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t group)
+{
+    return with_dim(cache.head_dim, [&](auto dp) -> uint64_t {
+        constexpr int DP = decltype(dp)::value;
+        uint64_t floats = attn::Part<attn::kSplitRows, DP>::FLOATS;
+        if (wants_tiles(cache, seqs, total_new, group)) floats = std::max<uint64_t>(floats, attn::Part<attn::TileCfg<DP>::ROWS, DP>::FLOATS);
+        return (uint64_t)rt->sm_count * 2 * floats * sizeof(float);
+    });
 }
 
 template <int DP>
@@ -38,6 +57,29 @@ Result launch_split(TesslRuntime *rt, Params p)
     TESSL_TRY(launch_pdl(rt, what, kernel, dim3(p.parts), dim3(C::THREADS), C::SMEM, p));
     return launch_pdl(rt, what, attn::attn_paged_combine_kernel<attn::kSplitRows, attn::kSplitUnit, DP, 4>, dim3(p.parts - 1, attn::kSplitRows / 4),
                       dim3(128), 0, p);
+}
+
+template <int DP>
+Result launch_tiles(TesslRuntime *rt, Params p, bool negate)
+{
+    using C = attn::TileCfg<DP>;
+    const char *what = "attn_paged tile launch";
+    auto kernel = attn::attn_paged_tile_kernel<DP>;
+    TESSL_TRY(smem_opt_in(rt, (const void *)kernel, C::SMEM, what, true));
+    EncodeTiled enc;
+    TESSL_TRY(tensormap_encoder(rt, what, &enc));
+    attn::TileParams tp{p, box_of(p.cache.page_size), negate};
+    tp.p.parts = (uint32_t)rt->sm_count;
+    tp.p.min_units = 4;
+    const cuuint64_t dims[4] = {p.cache.head_dim, p.cache.n_kv_heads, p.cache.page_size, p.cache.num_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)p.cache.head_stride * 2, (cuuint64_t)p.cache.token_stride * 2, p.cache.page_stride * 2};
+    const cuuint32_t box[4] = {64, 1, tp.box, 1};
+    CUtensorMap map_k, map_v;
+    TESSL_TRY(make_map(enc, what, &map_k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.cache.k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B));
+    TESSL_TRY(make_map(enc, what, &map_v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.cache.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B));
+    TESSL_TRY(launch_pdl(rt, what, kernel, dim3(tp.p.parts), dim3(C::THREADS), C::SMEM, map_k, map_v, tp));
+    return launch_pdl(rt, what, attn::attn_paged_combine_kernel<C::ROWS, attn::kTileKeys, DP, 32>, dim3(tp.p.parts - 1, C::ROWS / 32), dim3(128), 0,
+                      tp.p);
 }
 
 Result attn_params(const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t n_heads, const char *what, Params *p)
@@ -57,11 +99,10 @@ namespace nn {
 
 uint64_t attn_paged_workspace_bytes(TesslRuntime *rt, uint32_t total_new, uint32_t n_heads, const TesslPagedKv &cache, const TesslPagedSeqs &seqs)
 {
-    (void)seqs;
     if (cache.head_dim == 0 || cache.head_dim % 8 != 0 || cache.head_dim > 256 || cache.n_kv_heads == 0 || n_heads == 0 ||
         n_heads % cache.n_kv_heads != 0 || elems(total_new, n_heads) > 0x7fffffffull)
         return 0;
-    return workspace_of(rt, cache.head_dim);
+    return workspace_of(rt, cache, seqs, total_new, n_heads / cache.n_kv_heads);
 }
 
 Result attn_paged(TesslRuntime *rt, const TesslBuf &q, const TesslPagedKv &cache, const TesslPagedSeqs &seqs, const TesslBuf &out,
@@ -79,7 +120,7 @@ Result attn_paged(TesslRuntime *rt, const TesslBuf &q, const TesslPagedKv &cache
     TESSL_TRY(require_aligned16(q, "attn_paged q"));
     TESSL_TRY(require_aligned16(out, "attn_paged out"));
     if (q_stride % 8 != 0) return fmt("%s: rows of q are %u apart, not a multiple of 8", what, q_stride);
-    const uint64_t need = workspace_of(rt, cache.head_dim);
+    const uint64_t need = workspace_of(rt, cache, seqs, total_new, p.group);
     if (workspace.nbytes < need) return fmt("%s: the workspace has %llu bytes, the call needs %llu", what, (unsigned long long)workspace.nbytes, (unsigned long long)need);
     TESSL_TRY(require_aligned16(workspace, "attn_paged workspace"));
     if (!workspace.ptr) return fmt("%s: null workspace", what);
@@ -90,14 +131,17 @@ Result attn_paged(TesslRuntime *rt, const TesslBuf &q, const TesslPagedKv &cache
     if (total_new == 0 || seqs.num_seqs == 0) return ok();
     p.q = static_cast<const uint16_t *>(q.ptr), p.out = static_cast<uint16_t *>(out.ptr), p.work = static_cast<float *>(workspace.ptr);
     p.q_stride = q_stride;
-    p.scale_log2 = scale * 1.4426950408889634f;
     p.causal = causal, p.window = window, p.status = rt->status_dev;
-    switch (padded_dim(cache.head_dim)) {
-    case 64: return launch_split<64>(rt, p);
-    case 128: return launch_split<128>(rt, p);
-    case 192: return launch_split<192>(rt, p);
-    default: return launch_split<256>(rt, p);
-    }
+    p.scale_log2 = scale * 1.4426950408889634f;
+    // A scale of zero makes zeros of scores that a mask has set to -inf: the tile kernel masks before it scales.
+    const bool tiles = wants_tiles(cache, seqs, total_new, p.group) && p.scale_log2 != 0.0f;
+    return with_dim(cache.head_dim, [&](auto dp) {
+        constexpr int DP = decltype(dp)::value;
+        if (!tiles) return launch_split<DP>(rt, p);
+        const bool negate = p.scale_log2 < 0.0f;
+        p.scale_log2 = std::fabs(p.scale_log2);
+        return launch_tiles<DP>(rt, p, negate);
+    });
 }
 
 }  // namespace nn

@@ -59,33 +59,40 @@ __device__ __forceinline__ void key_range(const Params &p, const Seq &q, uint32_
     }
 }
 
-/// How a sequence divides: blocks of ROWS rows, units of UNIT keys from `first` on for each of them.
-struct Extent {
-    uint32_t blocks, units, first;
-};
+/// The keys of the item of rows block * ROWS ..: its first unit and how many units it has, one at least (rows that see nothing are
+/// written too).
 template <uint32_t ROWS, uint32_t UNIT>
-__device__ __forceinline__ Extent extent_of(const Params &p, const Seq &q)
+__device__ __forceinline__ void block_units(const Params &p, const Seq &q, uint32_t block, uint32_t &first, uint32_t &units)
 {
-    Extent e{0, 0, 0};
-    if (q.news == 0) return e;
+    const uint32_t rows = q.news * p.group, r0 = block * ROWS;
     uint32_t lo, hi;
-    key_range(p, q, 0, q.news - 1, lo, hi);
-    e.blocks = (uint32_t)(((uint64_t)q.news * p.group + ROWS - 1) / ROWS);
-    e.first = lo / UNIT * UNIT;
-    e.units = max(1u, (hi - e.first + UNIT - 1) / UNIT);  // rows that see nothing are written too
-    return e;
+    key_range(p, q, r0 / p.group, (min(r0 + ROWS, rows) - 1) / p.group, lo, hi);
+    first = lo / UNIT;
+    units = max(1u, (hi + UNIT - 1) / UNIT - first);
 }
-template <uint32_t ROWS, uint32_t UNIT>
-__device__ __forceinline__ uint64_t cost_of(const Params &p, uint32_t s)
+template <uint32_t ROWS>
+__device__ __forceinline__ uint32_t blocks_of(const Params &p, const Seq &q)
 {
-    const Extent e = extent_of<ROWS, UNIT>(p, seq_at(p, s));
-    return (uint64_t)e.blocks * e.units * p.cache.n_kv_heads;
+    return (q.news * p.group + ROWS - 1) / ROWS;
 }
 
-/// The line of units and how it is cut.
+/// An item, and where in it a part begins.
+struct Cursor {
+    Seq seq;
+    uint32_t kv_head, blocks, block, first, units, u0;
+};
+
+/// The line of units (key heads, in each the sequences, in each the blocks of rows) and how it is cut.
+template <uint32_t ROWS, uint32_t UNIT, uint32_t THREADS>
 struct Line {
-    uint64_t total;
+    struct Shared {
+        uint64_t warp_sum[THREADS / 32], cost[THREADS];
+        uint32_t many[THREADS], n_many, found;
+        uint64_t found_at;
+    };
+    uint64_t per_head, total;
     uint32_t parts;
+
     __device__ __forceinline__ uint64_t cut(uint32_t c) const { return total / parts * c + total % parts * c / parts; }
     /// The part that holds unit u.
     __device__ __forceinline__ uint32_t part_of(uint64_t u) const
@@ -95,74 +102,143 @@ struct Line {
         while (c + 1 < parts && cut(c + 1) <= u) ++c;
         return c;
     }
+
+    /// Units in front of this thread's sequence s0 + threadIdx.x among those of the block, its own in `mine`, all in `sum`.
+    /// Sequences of many blocks of rows are counted by a warp each.
+    static __device__ uint64_t scan(const Params &p, uint32_t s0, Shared &sh, uint64_t &mine, uint64_t &sum)
+    {
+        const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = s0 + tid;
+        __syncthreads();  // sh may still be read
+        if (tid == 0) sh.n_many = 0;
+        __syncthreads();
+        uint64_t cost = 0;
+        if (s < p.seqs.num_seqs) {
+            const Seq q = seq_at(p, s);
+            const uint32_t blocks = blocks_of<ROWS>(p, q);
+            if (blocks > 2) {
+                sh.many[atomicAdd(&sh.n_many, 1u)] = tid;
+            } else {
+                for (uint32_t b = 0; b < blocks; ++b) {
+                    uint32_t first, units;
+                    block_units<ROWS, UNIT>(p, q, b, first, units);
+                    cost += units;
+                }
+            }
+        }
+        sh.cost[tid] = cost;
+        __syncthreads();
+        for (uint32_t i = warp; i < sh.n_many; i += THREADS / 32) {
+            const uint32_t t = sh.many[i];
+            const Seq q = seq_at(p, s0 + t);
+            const uint32_t blocks = blocks_of<ROWS>(p, q);
+            uint64_t c = 0;
+            for (uint32_t b = lane; b < blocks; b += 32) {
+                uint32_t first, units;
+                block_units<ROWS, UNIT>(p, q, b, first, units);
+                c += units;
+            }
+#pragma unroll
+            for (uint32_t o = 16; o > 0; o /= 2) c += __shfl_xor_sync(0xffffffffu, c, o);
+            if (lane == 0) sh.cost[t] = c;
+        }
+        if (sh.n_many) __syncthreads();
+        mine = sh.cost[tid];
+        uint64_t run = mine;
+#pragma unroll
+        for (uint32_t o = 1; o < 32; o *= 2) {
+            const uint64_t t = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += t;
+        }
+        if (lane == 31) sh.warp_sum[warp] = run;
+        __syncthreads();
+        uint64_t before = 0;
+        sum = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < THREADS / 32; ++w) {
+            if (w < warp) before += sh.warp_sum[w];
+            sum += sh.warp_sum[w];
+        }
+        return before + run - mine;
+    }
+
+    /// The whole block calls this, and has one of: no part (false), or in `from` its place in the line and the item there. The
+    /// sequences are gone over twice where a block's threads do not hold them all.
+    __device__ bool start(const Params &p, uint32_t part, Shared &sh, uint64_t &from, Cursor &c)
+    {
+        const uint32_t n = p.seqs.num_seqs;
+        uint64_t mine, sum, at = scan(p, 0, sh, mine, sum);
+        per_head = sum;
+        for (uint32_t s0 = THREADS; s0 < n; s0 += THREADS) {
+            uint64_t m, t;
+            scan(p, s0, sh, m, t);
+            per_head += t;
+        }
+        total = per_head * p.cache.n_kv_heads;
+        parts = (uint32_t)min((uint64_t)p.parts, max((uint64_t)1, total / p.min_units));
+        if (part >= parts || total == 0) return false;
+        from = cut(part);
+        const uint64_t in_head = from % per_head;
+        c.kv_head = (uint32_t)(from / per_head);
+        uint64_t before = 0;
+        for (uint32_t s0 = 0; s0 < n; s0 += THREADS) {
+            if (n > THREADS) at = scan(p, s0, sh, mine, sum);
+            at += before;
+            if (at <= in_head && in_head < at + mine) sh.found = s0 + threadIdx.x, sh.found_at = at;
+            before += sum;
+            if (in_head < before) break;
+        }
+        __syncthreads();
+        c.seq = seq_at(p, sh.found);
+        c.blocks = blocks_of<ROWS>(p, c.seq);
+        uint64_t rest = in_head - sh.found_at;
+        const uint32_t lane = threadIdx.x & 31;
+        for (uint32_t b0 = 0;; b0 += 32) {  // every warp for itself
+            uint32_t first = 0, units = 0;
+            if (b0 + lane < c.blocks) block_units<ROWS, UNIT>(p, c.seq, b0 + lane, first, units);
+            uint64_t run = units;
+#pragma unroll
+            for (uint32_t o = 1; o < 32; o *= 2) {
+                const uint64_t t = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += t;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, run > rest);
+            if (past || b0 + 32 >= c.blocks) {
+                const uint32_t l = past ? __ffs(past) - 1 : 0;
+                c.block = b0 + l;
+                c.first = __shfl_sync(0xffffffffu, first, l), c.units = __shfl_sync(0xffffffffu, units, l);
+                c.u0 = (uint32_t)(rest - (__shfl_sync(0xffffffffu, run, l) - c.units));
+                break;
+            }
+            rest -= __shfl_sync(0xffffffffu, run, 31);
+        }
+        return true;
+    }
+
+    /// The item behind this one. Only where the line goes on.
+    static __device__ void next(const Params &p, Cursor &c)
+    {
+        c.u0 = 0;
+        if (++c.block >= c.blocks) {
+            c.block = 0;
+            do {
+                uint32_t s = c.seq.index + 1;
+                if (s >= p.seqs.num_seqs) s = 0, ++c.kv_head;
+                c.seq = seq_at(p, s);
+                c.blocks = blocks_of<ROWS>(p, c.seq);
+            } while (c.blocks == 0);
+        }
+        block_units<ROWS, UNIT>(p, c.seq, c.block, c.first, c.units);
+    }
 };
 
-/// Sum of v over the threads in front of this one, and over the block's in `total`.
-template <uint32_t THREADS>
-__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *scratch, uint64_t &total)
-{
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint64_t s = v;
-#pragma unroll
-    for (uint32_t o = 1; o < 32; o *= 2) {
-        const uint64_t t = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += t;
-    }
-    __syncthreads();  // scratch may still be read
-    if (lane == 31) scratch[warp] = s;
-    __syncthreads();
-    uint64_t before = 0;
-    total = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < THREADS / 32; ++w) {
-        if (w < warp) before += scratch[w];
-        total += scratch[w];
-    }
-    return before + s - v;
-}
-
-template <uint32_t ROWS, uint32_t UNIT, uint32_t THREADS>
-__device__ __forceinline__ Line line_of(const Params &p, uint64_t *scratch)
-{
-    uint64_t sum = 0;
-    for (uint32_t s = threadIdx.x; s < p.seqs.num_seqs; s += THREADS) sum += cost_of<ROWS, UNIT>(p, s);
-    Line l;
-    block_scan<THREADS>(sum, scratch, l.total);
-    l.parts = (uint32_t)min((uint64_t)p.parts, max((uint64_t)1, l.total / p.min_units));
-    return l;
-}
-
-/// The sequence that holds unit u of the line, and the unit at which it starts. The whole block calls this.
-template <uint32_t ROWS, uint32_t UNIT, uint32_t THREADS>
-__device__ __forceinline__ uint32_t seq_of_unit(const Params &p, uint64_t u, uint64_t *scratch, uint64_t &start)
-{
-    __shared__ uint32_t found;
-    __shared__ uint64_t found_start;
-    uint64_t before = 0;
-    if (threadIdx.x == 0) found = p.seqs.num_seqs;
-    for (uint32_t s0 = 0; s0 < p.seqs.num_seqs; s0 += THREADS) {
-        const uint32_t s = s0 + threadIdx.x;
-        const uint64_t cost = s < p.seqs.num_seqs ? cost_of<ROWS, UNIT>(p, s) : 0;
-        uint64_t total;
-        const uint64_t at = before + block_scan<THREADS>(cost, scratch, total);
-        if (at <= u && u < at + cost) found = s, found_start = at;
-        before += total;
-        __syncthreads();
-        if (u < before) break;
-    }
-    __syncthreads();
-    start = found_start;
-    const uint32_t s = found;
-    __syncthreads();
-    return s;
-}
-
-/// A part of an item in the workspace: 16 rows of DP unnormalised sums, then the rows' maxima (in powers of two) and sums.
+/// A part of an item in the workspace: ROWS rows of DP unnormalised sums, four columns of all rows after four of all rows, then
+/// the rows' maxima (in powers of two) and sums.
 template <uint32_t ROWS, uint32_t DP>
 struct Part {
-    static constexpr uint32_t FLOATS = ROWS * DP + 2 * ROWS;
+    static constexpr uint32_t FLOATS = ROWS * DP + 2 * ROWS, TOP = ROWS * DP, SUM = TOP + ROWS;
     /// `head`: the start of an item, else its middle or end.
     static __device__ __forceinline__ float *at(float *work, uint32_t part, bool head) { return work + ((size_t)part * 2 + head) * FLOATS; }
+    static __device__ __forceinline__ uint32_t four(uint32_t row, uint32_t col4) { return (col4 * ROWS + row) * 4; }
 };
 
 __device__ __forceinline__ float exp2_fast(float x)
@@ -186,52 +262,45 @@ __device__ __forceinline__ void row_at(const Params &p, const Seq &q, uint32_t k
     token += q.row0;
 }
 
-/// Adds up the parts of the items that cuts divide, one block per cut and ROWS_PER rows: the first cut in an item does it.
-template <uint32_t ROWS, uint32_t UNIT, uint32_t DP, uint32_t ROWS_PER>
+/// Adds up the parts of the items that cuts divide: a block per cut and RP rows, the first cut in an item does it. A thread has
+/// one row and every (THREADS / RP)-th four columns of it.
+template <uint32_t ROWS, uint32_t UNIT, uint32_t DP, uint32_t RP>
 __global__ void __launch_bounds__(128) attn_paged_combine_kernel(const Params p)
 {
     constexpr uint32_t THREADS = 128;
+    using L = Line<ROWS, UNIT, THREADS>;
+    using P = Part<ROWS, DP>;
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    __shared__ uint64_t scratch[THREADS / 32];
-    const Line l = line_of<ROWS, UNIT, THREADS>(p, scratch);
-    const uint32_t c = blockIdx.x + 1;
-    if (c >= l.parts) return;
-    const uint64_t u = l.cut(c);
-    uint64_t start;
-    const uint32_t s = seq_of_unit<ROWS, UNIT, THREADS>(p, u, scratch, start);
-    if (s >= p.seqs.num_seqs) return;
-    const Seq q = seq_at(p, s);
-    const Extent e = extent_of<ROWS, UNIT>(p, q);
-    const uint32_t item = (uint32_t)((u - start) / e.units);
-    const uint64_t from = start + (uint64_t)item * e.units, to = from + e.units;
-    if (u == from || l.cut(c - 1) > from) return;  // between two items; or an earlier cut is in this one
-    const uint32_t kv_head = item / e.blocks, block = item % e.blocks;
-    const uint32_t last = l.part_of(to - 1), rows = q.news * p.group, d = p.cache.head_dim;
-    constexpr uint32_t LANES = THREADS / ROWS_PER;  // per row
-    const uint32_t r = blockIdx.y * ROWS_PER + threadIdx.x / LANES, row = block * ROWS + r;
+    __shared__ typename L::Shared sh;
+    L l;
+    Cursor c;
+    uint64_t u;
+    const uint32_t part = blockIdx.x + 1;
+    if (!l.start(p, part, sh, u, c)) return;
+    const uint64_t from = u - c.u0, to = from + c.units;
+    if (c.u0 == 0 || l.cut(part - 1) > from) return;  // between two items; or an earlier cut is in this one
+    const uint32_t last = l.part_of(to - 1), rows = c.seq.news * p.group, d = p.cache.head_dim;
+    const uint32_t r = blockIdx.y * RP + threadIdx.x % RP, row = c.block * ROWS + r;
     if (row >= rows) return;
+    auto at = [&](uint32_t k) { return P::at(p.work, k, k == part - 1); };
     float m = -INFINITY;
-    for (uint32_t k = c - 1; k <= last; ++k) m = fmaxf(m, __ldcg(Part<ROWS, DP>::at(p.work, k, k == c - 1) + ROWS * DP + r));
+    for (uint32_t k = part - 1; k <= last; ++k) m = fmaxf(m, __ldcg(at(k) + P::TOP + r));
     const float top = m == -INFINITY ? 0.0f : m;
     float sum = 0.0f;
-    for (uint32_t k = c - 1; k <= last; ++k) {
-        const float *a = Part<ROWS, DP>::at(p.work, k, k == c - 1) + ROWS * DP + r;
-        sum += __ldcg(a + ROWS) * exp2_fast(__ldcg(a) - top);
-    }
+    for (uint32_t k = part - 1; k <= last; ++k) sum += __ldcg(at(k) + P::SUM + r) * exp2_fast(__ldcg(at(k) + P::TOP + r) - top);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     uint32_t token, head;
-    row_at(p, q, kv_head, row, token, head);
+    row_at(p, c.seq, c.kv_head, row, token, head);
     uint16_t *out = p.out + ((size_t)token * p.n_heads + head) * d;
-    for (uint32_t x = (threadIdx.x % LANES) * 4; x < d; x += LANES * 4) {
+    for (uint32_t x = threadIdx.x / RP; x * 4 < d; x += THREADS / RP) {
         float4 o = make_float4(0, 0, 0, 0);
-        for (uint32_t k = c - 1; k <= last; ++k) {
-            const float *a = Part<ROWS, DP>::at(p.work, k, k == c - 1);
-            const float f = exp2_fast(__ldcg(a + ROWS * DP + r) - top);
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(a + r * DP + x));
+        for (uint32_t k = part - 1; k <= last; ++k) {
+            const float f = exp2_fast(__ldcg(at(k) + P::TOP + r) - top);
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(at(k) + P::four(r, x)));
             o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
         }
-        *reinterpret_cast<uint2 *>(out + x) = make_uint2(bf16_pair(o.x * inv, o.y * inv), bf16_pair(o.z * inv, o.w * inv));
+        *reinterpret_cast<uint2 *>(out + x * 4) = make_uint2(bf16_pair(o.x * inv, o.y * inv), bf16_pair(o.z * inv, o.w * inv));
     }
 }
 

@@ -68,7 +68,6 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1) attn_paged_split_ker
     constexpr uint32_t ROWS = kSplitRows, UNIT = kSplitUnit;
     asm volatile("griddepcontrol.launch_dependents;");
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ uint64_t scratch[C::WARPS];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t ring = q4k::smem_u32(smem) + warp * C::RING;
     const uint32_t q_smem = q4k::smem_u32(smem) + C::WARPS * C::RING;
@@ -77,33 +76,24 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1) attn_paged_split_ker
     const uint32_t d = p.cache.head_dim, chunks = d / 8;
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    const Line line = line_of<ROWS, UNIT, C::THREADS>(p, scratch);
-    if (blockIdx.x >= line.parts) return;
-    uint64_t u = line.cut(blockIdx.x);
+    using L = Line<ROWS, UNIT, C::THREADS>;
+    __shared__ typename L::Shared shared;
+    L line;
+    Cursor cur;
+    uint64_t u;
+    if (!line.start(p, blockIdx.x, shared, u, cur)) return;
     const uint64_t u_end = line.cut(blockIdx.x + 1);
     if (u >= u_end) return;
-    uint64_t seq_start;
-    uint32_t s = seq_of_unit<ROWS, UNIT, C::THREADS>(p, u, scratch, seq_start);
-    if (s >= p.seqs.num_seqs) return;
-    Seq seq = seq_at(p, s);
-    Extent ext = extent_of<ROWS, UNIT>(p, seq);
 
     while (true) {
-        while (u - seq_start >= (uint64_t)ext.blocks * ext.units * p.cache.n_kv_heads) {  // the next sequence with new tokens
-            seq_start += (uint64_t)ext.blocks * ext.units * p.cache.n_kv_heads;
-            if (++s >= p.seqs.num_seqs) return;
-            seq = seq_at(p, s);
-            ext = extent_of<ROWS, UNIT>(p, seq);
-        }
-        const uint32_t item = (uint32_t)((u - seq_start) / ext.units), u0 = (uint32_t)((u - seq_start) % ext.units);
-        const uint32_t n_units = (uint32_t)min((uint64_t)(ext.units - u0), u_end - u);
-        const uint32_t kv_head = item / ext.blocks, block = item % ext.blocks;
-        const uint32_t rows = seq.news * p.group, row0 = block * ROWS;
+        const uint32_t n_units = (uint32_t)min((uint64_t)(cur.units - cur.u0), u_end - u);
+        const Seq &seq = cur.seq;
+        const uint32_t kv_head = cur.kv_head, u0 = cur.u0, rows = seq.news * p.group, row0 = cur.block * ROWS;
         // Keys of this part that the block's rows may see.
-        const uint32_t i0 = row0 / p.group, i1 = min(row0 + ROWS, rows) - 1;
+        const uint32_t i0 = row0 / p.group, i1 = (min(row0 + ROWS, rows) - 1) / p.group;
         uint32_t lo, hi;
-        key_range(p, seq, i0, i1 / p.group, lo, hi);
-        const uint32_t key0 = max(ext.first + u0 * UNIT, lo / kStep * kStep), key1 = min(ext.first + (u0 + n_units) * UNIT, hi);
+        key_range(p, seq, i0, i1, lo, hi);
+        const uint32_t key0 = max((cur.first + u0) * UNIT, lo / kStep * kStep), key1 = min((cur.first + u0 + n_units) * UNIT, hi);
         const uint32_t steps = key1 > key0 ? (key1 - key0 + kStep - 1) / kStep : 0;
         const uint32_t mine = steps > warp ? (steps - warp + C::WARPS - 1) / C::WARPS : 0;
 
@@ -119,7 +109,7 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1) attn_paged_split_ker
             asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(q_smem + chunk_at<DP>(r, cc)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
         }
 
-        const int32_t *table = p.seqs.table + (size_t)s * p.seqs.max_pages;
+        const int32_t *table = p.seqs.table + (size_t)seq.index * p.seqs.max_pages;
         const size_t head_off = (size_t)kv_head * p.cache.head_stride;
         // Lane l of a warp knows where key l % 16 of a step lies: -1 where there is none.
         auto locate = [&](uint32_t j) -> int64_t {
@@ -174,7 +164,7 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1) attn_paged_split_ker
         uint32_t lo_all, hi_all;  // what every row of the block sees
         {
             uint32_t t;
-            key_range(p, seq, i1 / p.group, i1 / p.group, lo_all, t);
+            key_range(p, seq, i1, i1, lo_all, t);
             key_range(p, seq, i0, i0, t, hi_all);
         }
 
@@ -274,8 +264,9 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1) attn_paged_split_ker
                     make_float2(o[n][2 * h] * f, o[n][2 * h + 1] * f);
         }
         __syncthreads();
-        const bool whole = n_units == ext.units;
-        float *part = Part<ROWS, DP>::at(p.work, blockIdx.x, u0 == 0);
+        const bool whole = n_units == cur.units;
+        using P = Part<ROWS, DP>;
+        float *part = P::at(p.work, blockIdx.x, u0 == 0);
         for (uint32_t c = tid; c < ROWS * (DP / 4); c += C::THREADS) {
             const uint32_t r = c / (DP / 4), x = c % (DP / 4);
             if (row0 + r >= rows || x * 4 >= d) continue;
@@ -299,12 +290,13 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1) attn_paged_split_ker
                 *reinterpret_cast<uint2 *>(p.out + ((size_t)token * p.n_heads + head) * d + x * 4) =
                     make_uint2(bf16_pair(sum.x * inv, sum.y * inv), bf16_pair(sum.z * inv, sum.w * inv));
             } else {
-                *reinterpret_cast<float4 *>(part + r * DP + x * 4) = sum;
-                if (x == 0) part[ROWS * DP + r] = t, part[ROWS * DP + ROWS + r] = den;
+                *reinterpret_cast<float4 *>(part + P::four(r, x)) = sum;
+                if (x == 0) part[P::TOP + r] = t, part[P::SUM + r] = den;
             }
         }
         u += n_units;
         if (u >= u_end) return;
+        L::next(p, cur);
         __syncthreads();  // rings, Q and ml are read
     }
 }
