@@ -40,9 +40,13 @@ struct TileCfg {
     static constexpr uint32_t CHUNK = 128 * 128, SLOT = CPS * CHUNK;  // bytes
     static constexpr uint32_t Q_BYTES = NT * CHUNKS * CHUNK;
     static constexpr uint32_t SLOTS = DP == 64 ? 11 : DP == 192 ? 3 : 5;
-    static constexpr uint32_t NBARS = 2 * SLOTS + NT * (2 * NS + 3) + 1;
+    static constexpr uint32_t BARS_T = 4 * NS + 2, NBARS = 2 * SLOTS + NT * BARS_T + 1;
     static constexpr uint32_t SMEM = Q_BYTES + SLOTS * SLOT + NBARS * 8 + 1024;  // + slack to align the base to 1 KiB
-    static constexpr uint32_t SOFTMAX_WARPS = 4 * NT, THREADS = (SOFTMAX_WARPS + 2) * 32;
+    // Two softmax warpgroups: a third one of the TMA and the MMA warp (and two that do nothing) gives them registers, 168 a
+    // thread at launch: 8 x 208 + 4 x 88 = 12 x 168.
+    static constexpr bool REGS = NT == 2;
+    static constexpr uint32_t SOFTMAX_WARPS = 4 * NT, THREADS = (SOFTMAX_WARPS + (REGS ? 4 : 2)) * 32;
+    static constexpr uint32_t POLY = NT == 2 ? 4 : 0;      // of 16 pairs of weights: 2^x by polynomial
     static constexpr uint32_t S_COL = 256;                 // TMEM columns: accumulators from 0, scores from here
     static_assert(SMEM <= 227 * 1024 - 64, "shared memory");
     static_assert(sizeof(typename Line<ROWS, kTileKeys, THREADS>::Shared) <= SLOTS * SLOT, "the scan of the line uses the ring");
@@ -52,7 +56,7 @@ struct TileCfg {
 struct TileParams {
     Params p;
     uint32_t box;      // tokens per TMA box
-    uint32_t negate;   // the scale is negative: q's signs are flipped instead
+    uint32_t negate;   // the scale is negative: the first product's A operand is negated instead
 };
 
 /// Box of the cache: 64 columns of one key head, `box` tokens of one page.
@@ -103,6 +107,50 @@ __device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&r)
         "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ uint64_t f32_pair(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void f32_unpair(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+/// The larger, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+/// 2^x of two finite values on the FMA pipe: x = n + f with n the nearest integer (Cody and Waite), 2^f by the polynomial of degree 4
+/// with the least relative error on [-1/2, 1/2] (Remez; 2.7e-6 in f32), n added to the exponent. Below 2^-126: 2^-126.
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t x)
+{
+    float a, b;
+    f32_unpair(x, a, b);
+    x = f32_pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are n
+    const uint64_t n = add2(x, f32_pair(kRound, kRound));
+    const uint64_t f = add2(x, fma2(n, f32_pair(-1.0f, -1.0f), f32_pair(kRound, kRound)));
+    uint64_t y = fma2(f, f32_pair(0.009570102207362652f, 0.009570102207362652f), f32_pair(0.05591785907745361f, 0.05591785907745361f));
+    y = fma2(y, f, f32_pair(0.240247443318367f, 0.240247443318367f));
+    y = fma2(y, f, f32_pair(0.6931217908859253f, 0.6931217908859253f));
+    y = fma2(y, f, f32_pair(0.9999992847442627f, 0.9999992847442627f));
+    float na, nb, ya, yb;
+    f32_unpair(n, na, nb), f32_unpair(y, ya, yb);
+    return f32_pair(__uint_as_float(__float_as_uint(ya) + (__float_as_uint(na) << 23)), __uint_as_float(__float_as_uint(yb) + (__float_as_uint(nb) << 23)));
+}
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -130,18 +178,20 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
     auto slot_full = [&](uint32_t s) { return bar0 + 8 * s; };
     auto slot_empty = [&](uint32_t s) { return bar0 + 8 * (C::SLOTS + s); };
     const uint32_t bar1 = bar0 + 16 * C::SLOTS;
-    auto s_full = [&](uint32_t t, uint32_t b) { return bar1 + 8 * (t * (2 * NS + 3) + b); };             // scores are there
-    auto p_full = [&](uint32_t t, uint32_t b) { return bar1 + 8 * (t * (2 * NS + 3) + NS + b); };        // weights are there, scores read
-    auto q_full = [&](uint32_t t) { return bar1 + 8 * (t * (2 * NS + 3) + 2 * NS); };
-    auto o_full = [&](uint32_t t) { return bar1 + 8 * (t * (2 * NS + 3) + 2 * NS + 1); };                // a product with V is done
-    auto o_free = [&](uint32_t t) { return bar1 + 8 * (t * (2 * NS + 3) + 2 * NS + 2); };                // the item's result is read
-    const uint32_t done = bar1 + 8 * (NT * (2 * NS + 3));
+    auto s_full = [&](uint32_t t, uint32_t b) { return bar1 + 8 * (t * C::BARS_T + b); };           // scores are there
+    auto p_full = [&](uint32_t t, uint32_t b) { return bar1 + 8 * (t * C::BARS_T + NS + b); };      // weights are there, scores read
+    // A product with V is done. One for each buffer of scores: products i and i + 1 may both be under way, i + 2 starts behind i's end.
+    auto o_full = [&](uint32_t t, uint32_t b) { return bar1 + 8 * (t * C::BARS_T + 2 * NS + b); };
+    auto p_half = [&](uint32_t t, uint32_t b) { return bar1 + 8 * (t * C::BARS_T + 3 * NS + b); };  // weights of the first 64 keys
+    auto q_full = [&](uint32_t t) { return bar1 + 8 * (t * C::BARS_T + 4 * NS); };
+    auto o_free = [&](uint32_t t) { return bar1 + 8 * (t * C::BARS_T + 4 * NS + 1); };              // the item's result is read
+    const uint32_t done = bar1 + 8 * (NT * C::BARS_T);
 
     if (warp == 0) {
         if (lane < C::SLOTS) mbar_init(slot_full(lane), 1), mbar_init(slot_empty(lane), 1);
         if (lane < NT) {
-            for (uint32_t b = 0; b < NS; ++b) mbar_init(s_full(lane, b), 1), mbar_init(p_full(lane, b), 4);
-            mbar_init(q_full(lane), 4), mbar_init(o_full(lane), 1), mbar_init(o_free(lane), 4);
+            for (uint32_t b = 0; b < NS; ++b) mbar_init(s_full(lane, b), 1), mbar_init(p_full(lane, b), 4), mbar_init(o_full(lane, b), 1), mbar_init(p_half(lane, b), 4);
+            mbar_init(q_full(lane), 4), mbar_init(o_free(lane), 4);
         }
         if (lane == 0) {
             abort_flag = 0;
@@ -190,8 +240,13 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
     auto v_place = [&](uint32_t j) { return j + min(n, j + NS); };
     uint32_t tiles = 0;  // of K and V, in front of the item
 
+    // Within its branch each, where the compiler can tell what holds.
+    auto fewer_regs = [] {
+        if constexpr (C::REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    };
     if (warp == C::SOFTMAX_WARPS) {
         // ------------------------------------------------ TMA ---
+        fewer_regs();
         const uint32_t boxes = kTileKeys / tp.box;
         uint32_t at = 0, phase = 0, issued = 0;  // ring position
         auto load = [&](const CUtensorMap *map, int page, int slot) -> bool {
@@ -254,9 +309,11 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
         __syncwarp();
     } else if (warp == C::SOFTMAX_WARPS + 1) {
         // ------------------------------------------------ MMA ---
+        fewer_regs();
         if (lane == 0) {
             constexpr uint32_t kBf16 = (1u << 4) | (1u << 7) | (1u << 10) | (8u << 24);  // f32 += bf16 . bf16, M = 128
-            constexpr uint32_t idesc_qk = kBf16 | ((kTileKeys >> 3) << 17), idesc_pv = kBf16 | (1u << 16) | ((C::CPS * 64 >> 3) << 17);
+            const uint32_t idesc_qk = kBf16 | ((kTileKeys >> 3) << 17) | (tp.negate << 13);  // -A
+            constexpr uint32_t idesc_pv = kBf16 | (1u << 16) | ((C::CPS * 64 >> 3) << 17);
             uint32_t used[NT], items[NT];  // tiles of scores, items of each row tile
             for (uint32_t t = 0; t < NT; ++t) used[t] = 0, items[t] = 0;
             bool ok = true;
@@ -298,22 +355,30 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                 for (uint32_t j = 0; j < n && ok; ++j) {
                     for (uint32_t t = 0; t < live; ++t) {
                         const uint32_t i = used[t] + j, buf = i % NS;
-                        if (!wait(p_full(t, buf), (i / NS) & 1u, 4)) break;
+                        if (!wait(p_half(t, buf), (i / NS) & 1u, 4)) break;
                         if (j == 0 && items[t] && !wait(o_free(t), (items[t] - 1) & 1u, 5)) break;
                         if (t == 0) wait_slots(v_place(j));
                         if (!ok) break;
                         pf::tcgen05_fence_after();
                         const uint32_t a = tmem + C::S_COL + (t * NS + buf) * 128, place = v_place(j);
 #pragma unroll
-                        for (uint32_t s = 0; s < C::SPT; ++s) {
-                            const uint32_t x = ((tiles + place) * C::SPT + s) % C::SLOTS;
-                            const uint64_t b = v_desc(ring + x * C::SLOT, C::CHUNK);
+                        for (uint32_t h = 0; h < 2; ++h) {  // the two halves of the keys
+                            if (h == 1) {
+                                if (!wait(p_full(t, buf), (i / NS) & 1u, 11)) break;
+                                pf::tcgen05_fence_after();
+                            }
 #pragma unroll
-                            for (uint32_t k = 0; k < kTileKeys / 16; ++k)
-                                tcgen05_mma_ts(tmem + t * DP + s * C::CPS * 64, a + 8 * k, b + k * (2048 >> 4), idesc_pv, j || k);
-                            if (t + 1 == live) pf::tcgen05_commit(slot_empty(x));
+                            for (uint32_t s = 0; s < C::SPT; ++s) {
+                                const uint32_t x = ((tiles + place) * C::SPT + s) % C::SLOTS;
+                                const uint64_t b = v_desc(ring + x * C::SLOT, C::CHUNK);
+#pragma unroll
+                                for (uint32_t k = h * kTileKeys / 32; k < (h + 1) * kTileKeys / 32; ++k)
+                                    tcgen05_mma_ts(tmem + t * DP + s * C::CPS * 64, a + 8 * k, b + k * (2048 >> 4), idesc_pv, j || k);
+                                if (h == 1 && t + 1 == live) pf::tcgen05_commit(slot_empty(x));
+                            }
                         }
-                        if (NS > 1 || j + 1 == n) pf::tcgen05_commit(o_full(t));
+                        if (!ok) break;
+                        if (NS > 1 || j + 1 == n) pf::tcgen05_commit(o_full(t, buf));
                         if (j + NS < n) {
                             if (t == 0) wait_slots(k_place(j + NS));
                             if (!ok) break;
@@ -334,13 +399,15 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                 if (clock64() - t0 > 4000000000ll) break;
         }
         __syncwarp();
-    } else {
+    } else if (warp < C::SOFTMAX_WARPS) {
         // ------------------------------------------------ softmax ---
+        if constexpr (C::REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const uint32_t t = warp >> 2, r = tid & 127;                     // row tile, row
         const uint32_t lanes = (warp & 3u) << 21;                        // this warp's quarter of the TMEM lanes
         const uint32_t o_tmem = tmem + lanes + t * DP, d = p.cache.head_dim;
         const float c2 = p.scale_log2;
-        uint32_t used = 0, o_seen = 0;
+        const uint64_t c2x2 = f32_pair(c2, c2);
+        uint32_t used = 0, items = 0;
         bool ok = true;
         // A whole warp's wait: every lane waits, all go on or none.
         auto wait = [&](uint32_t bar, uint32_t parity, uint32_t role, uint32_t where) {
@@ -348,28 +415,36 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
             if (!ok && lane == 0) fail(role, where);
             return ok;
         };
-        while (u < u_end && ok) {
-            item();
-            if (row0 + t * 128 < rows) {
-                if (n) {
-                    // Q: the last item's scores have been read, so nothing reads its Q any more
-                    for (uint32_t i = r; i < 128 * (DP / 8); i += 128) {
-                        const uint32_t qr = i / (DP / 8), cc = i % (DP / 8), row = row0 + t * 128 + qr;
-                        uint4 v = make_uint4(0, 0, 0, 0);
-                        if (row < rows && cc * 8 < d) {
-                            uint32_t token, head;
-                            row_at(p, cur.seq, cur.kv_head, row, token, head);
-                            v = __ldcg(reinterpret_cast<const uint4 *>(p.q + (size_t)token * p.q_stride + (size_t)head * d + cc * 8));
-                            if (tp.negate) v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
-                        }
-                        const uint32_t dst = q_smem + (t * C::CHUNKS + cc / 8) * C::CHUNK + qr * 128 + (((cc & 7u) ^ (qr & 7u)) << 4);
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-                    }
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(q_full(t));
-                }
-                const uint32_t row = row0 + t * 128 + r;
+        auto live = [&] { return u < u_end && row0 + t * 128 < rows; };  // the item at the cursor has rows here
+        // Q of the item at the cursor. The scores of the one before have been read, so nothing reads its Q any more.
+        auto load_q = [&] {
+            if (!live() || n == 0) return;
+            for (uint32_t i = r; i < 128 * (DP / 8); i += 128) {
+                const uint32_t qr = i / (DP / 8), cc = i % (DP / 8), row = row0 + t * 128 + qr;
+                const bool there = row < rows && cc * 8 < d;
+                uint32_t token = 0, head = 0;
+                if (there) row_at(p, cur.seq, cur.kv_head, row, token, head);
+                const uint32_t dst = q_smem + (t * C::CHUNKS + cc / 8) * C::CHUNK + qr * 128 + (((cc & 7u) ^ (qr & 7u)) << 4);
+                cp_async16(dst, p.q + (there ? (size_t)token * p.q_stride + (size_t)head * d + cc * 8 : 0), there);
+            }
+            cp_async_commit();
+        };
+        auto q_ready = [&] {
+            if (!live() || n == 0) return;
+            cp_async_wait<0>();
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full(t));
+        };
+        if (u < u_end) item();
+        load_q();
+        q_ready();
+        while (u < u_end) {
+            const bool mine = live();
+            const uint32_t row = row0 + t * 128 + r, tiles_n = n;
+            float top = -INFINITY, sum = 0.0f;  // raw score that the weights refer to; of the weights
+            uint16_t *out = nullptr;
+            if (mine) {
                 uint32_t lo_r, hi_r;  // rows past the last see what that sees
                 {
                     const uint32_t i = min(row, rows - 1) / p.group;
@@ -382,7 +457,6 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                     return j < n && key < cur.seq.keys && (uint32_t)__ldcg(table + key / p.cache.page_size) >= p.cache.num_pages;
                 };
                 bool hole = missing(0);
-                float top = -INFINITY, sum = 0.0f;  // raw score that the weights refer to; of the weights
                 for (uint32_t j = 0; j < n; ++j) {
                     const uint32_t buf = (used + j) % NS, key = k0 + j * kTileKeys;
                     const uint32_t s_tmem = tmem + lanes + C::S_COL + (t * NS + buf) * 128;
@@ -393,7 +467,8 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                     uint32_t s[2][64];
                     tmem_ld64(s_tmem, s[0]);
                     tmem_ld64(s_tmem + 64, s[1]);
-                    if (holes || key < lo_all || key + kTileKeys > hi_all) {
+                    const bool masked = holes || key < lo_all || key + kTileKeys > hi_all;
+                    if (masked) {
 #pragma unroll
                         for (uint32_t x = 0; x < 128; ++x)
                             if (key + x < lo_r || key + x >= hi_r || ((holes >> (x / 4)) & 1u)) s[x / 64][x % 64] = 0xff800000u;
@@ -403,14 +478,14 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                     for (uint32_t x = 0; x < 128; x += 8)
 #pragma unroll
                         for (uint32_t y = 0; y < 4; ++y)
-                            m4[y] = fmaxf(m4[y], fmaxf(__uint_as_float(s[x / 64][x % 64 + 2 * y]), __uint_as_float(s[x / 64][x % 64 + 2 * y + 1])));
-                    const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                    const bool grow = (m - top) * c2 > 8.0f;  // never where both are -inf
+                            m4[y] = max_nan(m4[y], max_nan(__uint_as_float(s[x / 64][x % 64 + 2 * y]), __uint_as_float(s[x / 64][x % 64 + 2 * y + 1])));
+                    const float m = max_nan(max_nan(m4[0], m4[1]), max_nan(m4[2], m4[3]));
+                    const bool grow = (m - top) * c2 > 8.0f;  // never where both are -inf, or m is NaN
                     if (__any_sync(0xffffffffu, grow)) {
                         const float f = grow ? exp2_fast((top - m) * c2) : 1.0f;
                         if (__any_sync(0xffffffffu, grow && top != -INFINITY)) {
                             // With one buffer the scores came behind the last product with V; with two, that may still run.
-                            if (NS > 1 && !wait(o_full(t), (o_seen + j - 1) & 1u, 7, j)) break;
+                            if (NS > 1 && !wait(o_full(t, (used + j - 1) % NS), ((used + j - 1) / NS) & 1u, 7, j)) break;
                             pf::tcgen05_fence_after();
 #pragma unroll 1
                             for (uint32_t x = 0; x < DP; x += 32) {
@@ -423,20 +498,6 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                         }
                         if (grow) sum *= f, top = m;
                     }
-                    const float off = top == -INFINITY ? 0.0f : -top * c2;
-                    float s4[4] = {0, 0, 0, 0};
-#pragma unroll
-                    for (uint32_t h = 0; h < 2; ++h) {
-                        uint32_t w[32];
-#pragma unroll
-                        for (uint32_t x = 0; x < 32; ++x) {
-                            const float a = exp2_fast(fmaf(__uint_as_float(s[h][2 * x]), c2, off)), b = exp2_fast(fmaf(__uint_as_float(s[h][2 * x + 1]), c2, off));
-                            s4[2 * (x & 1)] += a, s4[2 * (x & 1) + 1] += b;
-                            w[x] = bf16_pair(a, b);
-                        }
-                        tmem_store32(s_tmem + h * 32, w);
-                    }
-                    sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
                     if (key + kTileKeys > cur.seq.keys) {  // slots behind the sequence: no values
                         for (uint32_t i = 0; i < C::SPT; ++i) {
                             const uint32_t x = (tiles + v_place(j)) * C::SPT + i, slot = ring + x % C::SLOTS * C::SLOT;
@@ -449,66 +510,105 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                         __syncwarp();
                         if (!ok) break;
                     }
-                    tmem_store_wait();
-                    pf::tcgen05_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(p_full(t, buf));
+                    const float off = top == -INFINITY ? 0.0f : -top * c2;
+                    const uint64_t offx2 = f32_pair(off, off);
+                    // The polynomial knows neither infinities nor NaN: rows with any, and masked tiles, do without it.
+                    const bool plain = masked || __any_sync(0xffffffffu, !(m < INFINITY) || top == -INFINITY);
+                    uint64_t s2[2] = {0, 0};
+                    auto half = [&](uint32_t h, auto poly) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (uint32_t x = 0; x < 32; ++x) {
+                            const uint64_t y = fma2(f32_pair(__uint_as_float(s[h][2 * x]), __uint_as_float(s[h][2 * x + 1])), c2x2, offx2);
+                            uint64_t e;
+                            if (decltype(poly)::value && (int)(x % 16) < (int)C::POLY) {
+                                e = exp2_poly(y);
+                            } else {
+                                float a, b;
+                                f32_unpair(y, a, b);
+                                e = f32_pair(exp2_fast(a), exp2_fast(b));
+                            }
+                            s2[x & 1] = add2(s2[x & 1], e);
+                            float a, b;
+                            f32_unpair(e, a, b);
+                            w[x] = bf16_pair(a, b);
+                        }
+                        tmem_store32(s_tmem + h * 32, w);
+                        tmem_store_wait();
+                        pf::tcgen05_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(h == 0 ? p_half(t, buf) : p_full(t, buf));
+                    };
+                    if (plain || C::POLY == 0) {
+                        half(0, std::false_type{}), half(1, std::false_type{});
+                    } else {
+                        half(0, std::true_type{}), half(1, std::true_type{});
+                    }
+                    float a, b;
+                    f32_unpair(add2(s2[0], s2[1]), a, b);
+                    sum += a + b;
                 }
                 if (!ok) break;
-                if (n) {
-                    // With two buffers of scores the last two products may both be under way, and a barrier tells one phase from the next only.
-                    if (NS > 1 && n > 1 && !wait(o_full(t), (o_seen + n - 2) & 1u, 9, n)) break;
-                    if (!wait(o_full(t), (NS > 1 ? o_seen + n - 1 : o_seen) & 1u, 10, n)) break;
-                    pf::tcgen05_fence_after();
-                    o_seen += NS > 1 ? n : 1;
-                    used += n;
-                }
-                const bool whole = n_units == cur.units;
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                float *part = P::at(p.work, blockIdx.x, cur.u0 == 0);
-                uint32_t token = 0, head = 0;
-                if (row < rows) row_at(p, cur.seq, cur.kv_head, row, token, head);
-                uint16_t *out = p.out + ((size_t)token * p.n_heads + head) * d;
-#pragma unroll 1
-                for (uint32_t x = 0; x < DP; x += 32) {
-                    if (x >= d) break;
-                    uint32_t o[32];
-                    if (n) {
-                        pf::tmem_ld32(o_tmem + x, o);
-                    } else {
-#pragma unroll
-                        for (int y = 0; y < 32; ++y) o[y] = 0;
-                    }
-                    if (row < rows && whole) {
-#pragma unroll
-                        for (uint32_t y = 0; y < 32; y += 8) {
-                            if (x + y >= d) break;
-                            uint4 v;
-                            v.x = bf16_pair(__uint_as_float(o[y]) * inv, __uint_as_float(o[y + 1]) * inv);
-                            v.y = bf16_pair(__uint_as_float(o[y + 2]) * inv, __uint_as_float(o[y + 3]) * inv);
-                            v.z = bf16_pair(__uint_as_float(o[y + 4]) * inv, __uint_as_float(o[y + 5]) * inv);
-                            v.w = bf16_pair(__uint_as_float(o[y + 6]) * inv, __uint_as_float(o[y + 7]) * inv);
-                            *reinterpret_cast<uint4 *>(out + x + y) = v;
-                        }
-                    } else if (row < rows) {
-#pragma unroll
-                        for (uint32_t y = 0; y < 32; y += 4)
-                            *reinterpret_cast<uint4 *>(part + P::four(t * 128 + r, (x + y) / 4)) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
-                    }
-                    __syncwarp();
-                }
-                if (!whole && row < rows) part[P::TOP + t * 128 + r] = top == -INFINITY ? top : top * c2, part[P::SUM + t * 128 + r] = sum;
-                if (n) {
-                    pf::tcgen05_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(o_free(t));
+                used += n;
+                if (row < rows) {
+                    uint32_t token, head;
+                    row_at(p, cur.seq, cur.kv_head, row, token, head);
+                    out = p.out + ((size_t)token * p.n_heads + head) * d;
                 }
             }
+            const bool whole = n_units == cur.units;
+            float *part = P::at(p.work, blockIdx.x, cur.u0 == 0);
             tiles += 2 * n;
             u += n_units;
-            if (u < u_end) L::next(p, cur);
+            if (u < u_end) L::next(p, cur), item();
+            load_q();  // of the next item, while the last product runs
+            if (mine && tiles_n) {
+                const uint32_t last = used - 1;
+                if (!wait(o_full(t, last % NS), (NS > 1 ? last / NS : items) & 1u, 9, 0)) break;
+                pf::tcgen05_fence_after();
+                ++items;
+            }
+            q_ready();
+            if (!mine) continue;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll 1
+            for (uint32_t x = 0; x < DP; x += 32) {
+                if (x >= d) break;
+                uint32_t o[32];
+                if (tiles_n) {
+                    pf::tmem_ld32(o_tmem + x, o);
+                } else {
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) o[y] = 0;
+                }
+                if (out && whole) {
+#pragma unroll
+                    for (uint32_t y = 0; y < 32; y += 8) {
+                        if (x + y >= d) break;
+                        uint4 v;
+                        v.x = bf16_pair(__uint_as_float(o[y]) * inv, __uint_as_float(o[y + 1]) * inv);
+                        v.y = bf16_pair(__uint_as_float(o[y + 2]) * inv, __uint_as_float(o[y + 3]) * inv);
+                        v.z = bf16_pair(__uint_as_float(o[y + 4]) * inv, __uint_as_float(o[y + 5]) * inv);
+                        v.w = bf16_pair(__uint_as_float(o[y + 6]) * inv, __uint_as_float(o[y + 7]) * inv);
+                        *reinterpret_cast<uint4 *>(out + x + y) = v;
+                    }
+                } else if (out) {
+#pragma unroll
+                    for (uint32_t y = 0; y < 32; y += 4)
+                        *reinterpret_cast<uint4 *>(part + P::four(t * 128 + r, (x + y) / 4)) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+                }
+                __syncwarp();
+            }
+            if (!whole && out) part[P::TOP + t * 128 + r] = top == -INFINITY ? top : top * c2, part[P::SUM + t * 128 + r] = sum;
+            if (tiles_n) {
+                pf::tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(o_free(t));
+            }
         }
         __syncwarp();
+    } else {
+        fewer_regs();
     }
     pf::tcgen05_fence_before();
     __syncthreads();
