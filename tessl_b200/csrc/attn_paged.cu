@@ -78,7 +78,8 @@ Result launch_tiles(TesslRuntime *rt, Params p, bool negate)
     TESSL_TRY(make_map(enc, what, &map_k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.cache.k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B));
     TESSL_TRY(make_map(enc, what, &map_v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.cache.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B));
     TESSL_TRY(launch_pdl(rt, what, kernel, dim3(tp.p.parts), dim3(C::THREADS), C::SMEM, map_k, map_v, tp));
-    return launch_pdl(rt, what, attn::attn_paged_combine_kernel<C::ROWS, attn::kTileKeys, DP, 32>, dim3(tp.p.parts - 1, C::ROWS / 32), dim3(128), 0,
+    constexpr uint32_t RP = DP <= 128 ? 32 : 16;
+    return launch_pdl(rt, what, attn::attn_paged_combine_kernel<C::ROWS, attn::kTileKeys, DP, RP>, dim3(tp.p.parts - 1, C::ROWS / RP), dim3(128), 0,
                       tp.p);
 }
 

@@ -284,23 +284,41 @@ __global__ void __launch_bounds__(128) attn_paged_combine_kernel(const Params p)
     const uint32_t r = blockIdx.y * RP + threadIdx.x % RP, row = c.block * ROWS + r;
     if (row >= rows) return;
     auto at = [&](uint32_t k) { return P::at(p.work, k, k == part - 1); };
-    float m = -INFINITY;
-    for (uint32_t k = part - 1; k <= last; ++k) m = fmaxf(m, __ldcg(at(k) + P::TOP + r));
-    const float top = m == -INFINITY ? 0.0f : m;
-    float sum = 0.0f;
-    for (uint32_t k = part - 1; k <= last; ++k) sum += __ldcg(at(k) + P::SUM + r) * exp2_fast(__ldcg(at(k) + P::TOP + r) - top);
+    constexpr uint32_t NX = (DP / 4 + THREADS / RP - 1) / (THREADS / RP);  // fours of columns of a thread
+    const uint32_t x0 = threadIdx.x / RP;
+    // One pass over the parts, in the order of the keys, the sums scaled when the maximum grows: a part's loads are issued together.
+    float m = -INFINITY, sum = 0.0f;
+    float4 o[NX];
+#pragma unroll
+    for (uint32_t i = 0; i < NX; ++i) o[i] = make_float4(0, 0, 0, 0);
+#pragma unroll 2
+    for (uint32_t k = part - 1; k <= last; ++k) {
+        const float *a = at(k);
+        const float top = __ldcg(a + P::TOP + r), den = __ldcg(a + P::SUM + r);
+        float4 v[NX];
+#pragma unroll
+        for (uint32_t i = 0; i < NX; ++i) {
+            const uint32_t x = x0 + i * (THREADS / RP);
+            if (x * 4 < d) v[i] = __ldcg(reinterpret_cast<const float4 *>(a + P::four(r, x)));
+        }
+        const float all = fmaxf(m, top), ref = all == -INFINITY ? 0.0f : all;
+        const float f = exp2_fast(m - ref), g = exp2_fast(top - ref);
+        m = all;
+        sum = sum * f + den * g;
+#pragma unroll
+        for (uint32_t i = 0; i < NX; ++i) {
+            o[i].x = o[i].x * f + v[i].x * g, o[i].y = o[i].y * f + v[i].y * g;
+            o[i].z = o[i].z * f + v[i].z * g, o[i].w = o[i].w * f + v[i].w * g;
+        }
+    }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     uint32_t token, head;
     row_at(p, c.seq, c.kv_head, row, token, head);
     uint16_t *out = p.out + ((size_t)token * p.n_heads + head) * d;
-    for (uint32_t x = threadIdx.x / RP; x * 4 < d; x += THREADS / RP) {
-        float4 o = make_float4(0, 0, 0, 0);
-        for (uint32_t k = part - 1; k <= last; ++k) {
-            const float f = exp2_fast(__ldcg(at(k) + P::TOP + r) - top);
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(at(k) + P::four(r, x)));
-            o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
-        }
-        *reinterpret_cast<uint2 *>(out + x * 4) = make_uint2(bf16_pair(o.x * inv, o.y * inv), bf16_pair(o.z * inv, o.w * inv));
+#pragma unroll
+    for (uint32_t i = 0; i < NX; ++i) {
+        const uint32_t x = x0 + i * (THREADS / RP);
+        if (x * 4 < d) *reinterpret_cast<uint2 *>(out + x * 4) = make_uint2(bf16_pair(o[i].x * inv, o[i].y * inv), bf16_pair(o[i].z * inv, o[i].w * inv));
     }
 }
 

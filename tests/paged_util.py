@@ -85,7 +85,7 @@ class Batch:
         Tolerance: the result's rounding to bf16 (U16 of it); the weights' rounding to bf16 (U16 of sum p |v| / sum p); a score is a sum
         of dim products in f32 and one multiplication (each step off by U32 of the sum of magnitudes, twice that for a sum that
         truncates), an error of a weight's exponent and so a relative one of the weight, which counts in the sum and in the divisor; the
-        exponential (2^-18, in both) and the f32 sums over the keys and the parts (U32 a step)."""
+        exponential (2^-21, in both) and the f32 sums over the keys and the parts (U32 a step)."""
         scale = self.dim ** -0.5 if scale is None else scale
         out, tol = np.zeros((self.live, self.heads, self.dim)), np.zeros((self.live, self.heads, self.dim))
         for s in range(self.n):
@@ -113,7 +113,7 @@ class Batch:
                 den[den == 0] = 1.0
                 o, a = (w @ v[:, e]) / den, (w @ np.abs(v[:, e])) / den
                 mag = np.where(seen, abs(scale) * (np.abs(q) @ np.abs(k[:, e]).T), 0.0).max(axis=1, keepdims=True)
-                off = 2 * (self.dim + 8) * 2 * U32 * mag + 2 * 2.0 ** -18 + (n + 64) * 2 * U32
+                off = 2 * (self.dim + 8) * 2 * U32 * mag + 2 * 2.0 ** -21 + (n + 64) * 2 * U32
                 out[row0:row0 + self.news[s], h] = o
                 tol[row0:row0 + self.news[s], h] = U16 * np.abs(o) * (1 + U16) + (U16 + off) * a * (1 + U16) + 1e-30
         return out, tol
