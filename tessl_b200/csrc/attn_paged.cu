@@ -1,6 +1,7 @@
 // Attention over a paged cache: checks, routes and launches.
 #include <algorithm>
 #include <cmath>
+#include <random>
 #include <type_traits>
 
 #include "attn_paged_split.cuh"
@@ -26,61 +27,82 @@ auto with_dim(uint32_t head_dim, F f)
     }
 }
 
-/// Tokens per TMA box: a power of two that divides a page; fewer than eight would break the swizzle's groups of eight rows.
-uint32_t box_of(uint32_t page_size) { return std::min(page_size & (0u - page_size), attn::kTileKeys); }
+/// Tokens per TMA box, of those that a step or tile of keys has: a power of two that divides a page; fewer than eight would break the
+/// swizzle's groups of eight rows.
+uint32_t box_of(uint32_t page_size, uint32_t most) { return std::min(page_size & (0u - page_size), most); }
 
 /// Whether a call of these sizes goes to the tensor-core tiles: enough rows for each key head of a sequence to fill some of a tile.
 bool wants_tiles(const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t group)
 {
-    return seqs.q_starts.ptr && cache.num_pages > 0 && box_of(cache.page_size) >= 8 && elems(total_new, group) > 32ull * seqs.num_seqs;
+    return seqs.q_starts.ptr && cache.num_pages > 0 && cache.page_size % 8 == 0 && elems(total_new, group) > 32ull * seqs.num_seqs;
 }
 
 uint64_t workspace_of(const TesslRuntime *rt, const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t group)
 {
     return with_dim(cache.head_dim, [&](auto dp) -> uint64_t {
         constexpr int DP = decltype(dp)::value;
-        uint64_t floats = attn::Part<attn::kSplitRows, DP>::FLOATS;
-        if (wants_tiles(cache, seqs, total_new, group)) floats = std::max<uint64_t>(floats, attn::Part<attn::TileCfg<DP>::ROWS, DP>::FLOATS);
-        return (uint64_t)rt->sm_count * 2 * floats * sizeof(float);
+        const uint64_t few = attn::Part<attn::kSplitRows, DP>::bytes(rt->sm_count), many = attn::Part<attn::TileCfg<DP>::ROWS, DP>::bytes(rt->sm_count);
+        return wants_tiles(cache, seqs, total_new, group) ? std::max(few, many) : few;
     });
 }
 
-template <int DP>
-Result launch_split(TesslRuntime *rt, Params p)
+/// The cache's maps for boxes of 64 columns of one key head and `box` tokens of one page.
+Result cache_maps(TesslRuntime *rt, const char *what, const paged::Cache &c, uint32_t box, CUtensorMap *k, CUtensorMap *v)
 {
-    using C = attn::SplitCfg<DP>;
-    const char *what = "attn_paged launch";
-    auto kernel = attn::attn_paged_split_kernel<DP>;
-    TESSL_TRY(smem_opt_in(rt, (const void *)kernel, C::SMEM, what, true));
-    p.parts = (uint32_t)rt->sm_count;
-    p.min_units = 2;
-    TESSL_TRY(launch_pdl(rt, what, kernel, dim3(p.parts), dim3(C::THREADS), C::SMEM, p));
-    return launch_pdl(rt, what, attn::attn_paged_combine_kernel<attn::kSplitRows, attn::kSplitUnit, DP, 4>, dim3(p.parts - 1, attn::kSplitRows / 4),
-                      dim3(128), 0, p);
+    EncodeTiled enc;
+    TESSL_TRY(tensormap_encoder(rt, what, &enc));
+    const cuuint64_t dims[4] = {c.head_dim, c.n_kv_heads, c.page_size, c.num_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.head_stride * 2, (cuuint64_t)c.token_stride * 2, c.page_stride * 2};
+    const cuuint32_t boxes[4] = {64, 1, box, 1};
+    TESSL_TRY(make_map(enc, what, k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c.k, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_128B));
+    return make_map(enc, what, v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c.v, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int DP>
-Result launch_tiles(TesslRuntime *rt, Params p, bool negate)
+Result launch_split(TesslRuntime *rt, const Params &p)
+{
+    using C = attn::SplitCfg<DP>;
+    const char *what = "attn_paged launch";
+    attn::SplitParams sp{p, box_of(p.cache.page_size, attn::kStep)};
+    sp.p.parts = (uint32_t)rt->sm_count;
+    sp.p.min_units = 2;
+    CUtensorMap map_k{}, map_v{};
+    auto go = [&](auto kernel) -> Result {
+        TESSL_TRY(smem_opt_in(rt, (const void *)kernel, C::SMEM, what, true));
+        return launch_pdl(rt, what, kernel, dim3(sp.p.parts), dim3(C::THREADS), C::SMEM, map_k, map_v, sp);
+    };
+    if (p.cache.num_pages == 0 || sp.box < 8) return go(attn::attn_paged_split_kernel<DP, false>);
+    TESSL_TRY(cache_maps(rt, what, p.cache, sp.box, &map_k, &map_v));
+    return go(attn::attn_paged_split_kernel<DP, true>);
+}
+
+template <int DP>
+Result launch_tiles(TesslRuntime *rt, const Params &p, bool negate)
 {
     using C = attn::TileCfg<DP>;
     const char *what = "attn_paged tile launch";
     auto kernel = attn::attn_paged_tile_kernel<DP>;
     TESSL_TRY(smem_opt_in(rt, (const void *)kernel, C::SMEM, what, true));
-    EncodeTiled enc;
-    TESSL_TRY(tensormap_encoder(rt, what, &enc));
-    attn::TileParams tp{p, box_of(p.cache.page_size), negate};
+    attn::TileParams tp{p, box_of(p.cache.page_size, attn::kTileKeys), negate};
     tp.p.parts = (uint32_t)rt->sm_count;
     tp.p.min_units = 4;
-    const cuuint64_t dims[4] = {p.cache.head_dim, p.cache.n_kv_heads, p.cache.page_size, p.cache.num_pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)p.cache.head_stride * 2, (cuuint64_t)p.cache.token_stride * 2, p.cache.page_stride * 2};
-    const cuuint32_t box[4] = {64, 1, tp.box, 1};
     CUtensorMap map_k, map_v;
-    TESSL_TRY(make_map(enc, what, &map_k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.cache.k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B));
-    TESSL_TRY(make_map(enc, what, &map_v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.cache.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B));
-    TESSL_TRY(launch_pdl(rt, what, kernel, dim3(tp.p.parts), dim3(C::THREADS), C::SMEM, map_k, map_v, tp));
-    constexpr uint32_t RP = DP <= 128 ? 32 : 16;
-    return launch_pdl(rt, what, attn::attn_paged_combine_kernel<C::ROWS, attn::kTileKeys, DP, RP>, dim3(tp.p.parts - 1, C::ROWS / RP), dim3(128), 0,
-                      tp.p);
+    TESSL_TRY(cache_maps(rt, what, p.cache, tp.box, &map_k, &map_v));
+    return launch_pdl(rt, what, kernel, dim3(tp.p.parts), dim3(C::THREADS), C::SMEM, map_k, map_v, tp);
+}
+
+/// A number that no other call's parts are marked with: the n-th of a sequence that differs from runtime to runtime (splitmix64).
+uint64_t next_mark(TesslRuntime *rt)
+{
+    if (!rt->attn_mark) {
+        std::random_device random;
+        rt->attn_mark = ((uint64_t)random() << 32 | random()) ^ (uint64_t)(uintptr_t)rt;
+    }
+    uint64_t z = rt->attn_mark += 0x9e3779b97f4a7c15ull;
+    z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
+    z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
+    z ^= z >> 31;
+    return z ? z : 1;  // 0 is no mark
 }
 
 Result attn_params(const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t n_heads, const char *what, Params *p)
@@ -134,6 +156,7 @@ Result attn_paged(TesslRuntime *rt, const TesslBuf &q, const TesslPagedKv &cache
     p.q_stride = q_stride;
     p.causal = causal, p.window = window, p.status = rt->status_dev;
     p.scale_log2 = scale * 1.4426950408889634f;
+    p.mark = next_mark(rt);
     // A scale of zero makes zeros of scores that a mask has set to -inf: the tile kernel masks before it scales.
     const bool tiles = wants_tiles(cache, seqs, total_new, p.group) && p.scale_log2 != 0.0f;
     return with_dim(cache.head_dim, [&](auto dp) {

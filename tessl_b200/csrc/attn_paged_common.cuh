@@ -6,8 +6,9 @@
 // call, item after item, are one line that is cut into equal parts, one per block of the launch: whatever the lengths of the
 // sequences, every block reads the same number of keys. The lengths are on the device, so the blocks work the cuts out
 // themselves. A block that has an item to itself writes its rows; the parts of an item that a cut divides go to the workspace,
-// two at most per block (the end of one item, the start of another), and a second launch, one block per cut, adds them up in the
-// order of the keys: the same sums on every run.
+// two at most per block (the end of one item, the start of another). A block marks its parts when it is done and looks whether those
+// of the others are marked: the last one to come adds them up, in the order of the keys, the same sums on every run. (A second
+// launch for the sums took 9 us of the 18 of a token over 777 keys, and 21 of 74 of ragged chunks.)
 #pragma once
 #include "paged_common.cuh"
 #include "q4_gemv_tma.cuh"
@@ -26,6 +27,7 @@ struct Params {
     uint32_t causal, window;
     uint32_t parts;      // blocks that the line of units may be cut for
     uint32_t min_units;  // units that a part is worth
+    uint64_t mark;       // of this call's parts
     uint32_t *status;
 };
 
@@ -81,14 +83,20 @@ struct Cursor {
     Seq seq;
     uint32_t kv_head, blocks, block, first, units, u0;
 };
+/// An item of which a block has a part, and where the item begins on the line.
+struct Pending {
+    Cursor c;
+    uint64_t from;
+};
 
 /// The line of units (key heads, in each the sequences, in each the blocks of rows) and how it is cut.
 template <uint32_t ROWS, uint32_t UNIT, uint32_t THREADS>
 struct Line {
     struct Shared {
         uint64_t warp_sum[THREADS / 32], cost[THREADS];
-        uint32_t many[THREADS], n_many, found;
+        uint32_t many[THREADS], n_many;
         uint64_t found_at;
+        Seq found;
     };
     uint64_t per_head, total;
     uint32_t parts;
@@ -105,7 +113,7 @@ struct Line {
 
     /// Units in front of this thread's sequence s0 + threadIdx.x among those of the block, its own in `mine`, all in `sum`.
     /// Sequences of many blocks of rows are counted by a warp each.
-    static __device__ uint64_t scan(const Params &p, uint32_t s0, Shared &sh, uint64_t &mine, uint64_t &sum)
+    static __device__ uint64_t scan(const Params &p, uint32_t s0, Shared &sh, Seq &q, uint64_t &mine, uint64_t &sum)
     {
         const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = s0 + tid;
         __syncthreads();  // sh may still be read
@@ -113,7 +121,7 @@ struct Line {
         __syncthreads();
         uint64_t cost = 0;
         if (s < p.seqs.num_seqs) {
-            const Seq q = seq_at(p, s);
+            q = seq_at(p, s);
             const uint32_t blocks = blocks_of<ROWS>(p, q);
             if (blocks > 2) {
                 sh.many[atomicAdd(&sh.n_many, 1u)] = tid;
@@ -129,12 +137,12 @@ struct Line {
         __syncthreads();
         for (uint32_t i = warp; i < sh.n_many; i += THREADS / 32) {
             const uint32_t t = sh.many[i];
-            const Seq q = seq_at(p, s0 + t);
-            const uint32_t blocks = blocks_of<ROWS>(p, q);
+            const Seq r = seq_at(p, s0 + t);
+            const uint32_t blocks = blocks_of<ROWS>(p, r);
             uint64_t c = 0;
             for (uint32_t b = lane; b < blocks; b += 32) {
                 uint32_t first, units;
-                block_units<ROWS, UNIT>(p, q, b, first, units);
+                block_units<ROWS, UNIT>(p, r, b, first, units);
                 c += units;
             }
 #pragma unroll
@@ -165,13 +173,30 @@ struct Line {
     /// sequences are gone over twice where a block's threads do not hold them all.
     __device__ bool start(const Params &p, uint32_t part, Shared &sh, uint64_t &from, Cursor &c)
     {
-        const uint32_t n = p.seqs.num_seqs;
-        uint64_t mine, sum, at = scan(p, 0, sh, mine, sum);
-        per_head = sum;
-        for (uint32_t s0 = THREADS; s0 < n; s0 += THREADS) {
-            uint64_t m, t;
-            scan(p, s0, sh, m, t);
-            per_head += t;
+        const uint32_t n = p.seqs.num_seqs, lane = threadIdx.x & 31;
+        uint64_t mine, sum, at, found_at = 0;
+        Seq q;
+        if (n == 1) {  // every warp for itself
+            q = seq_at(p, 0);
+            const uint32_t blocks = blocks_of<ROWS>(p, q);
+            sum = 0;
+            for (uint32_t b = lane; b < blocks; b += 32) {
+                uint32_t first, units;
+                block_units<ROWS, UNIT>(p, q, b, first, units);
+                sum += units;
+            }
+#pragma unroll
+            for (uint32_t o = 16; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            per_head = sum;
+        } else {
+            at = scan(p, 0, sh, q, mine, sum);
+            per_head = sum;
+            for (uint32_t s0 = THREADS; s0 < n; s0 += THREADS) {
+                uint64_t m, t;
+                Seq other;
+                scan(p, s0, sh, other, m, t);
+                per_head += t;
+            }
         }
         total = per_head * p.cache.n_kv_heads;
         parts = (uint32_t)min((uint64_t)p.parts, max((uint64_t)1, total / p.min_units));
@@ -179,19 +204,21 @@ struct Line {
         from = cut(part);
         const uint64_t in_head = from % per_head;
         c.kv_head = (uint32_t)(from / per_head);
-        uint64_t before = 0;
-        for (uint32_t s0 = 0; s0 < n; s0 += THREADS) {
-            if (n > THREADS) at = scan(p, s0, sh, mine, sum);
-            at += before;
-            if (at <= in_head && in_head < at + mine) sh.found = s0 + threadIdx.x, sh.found_at = at;
-            before += sum;
-            if (in_head < before) break;
+        if (n > 1) {
+            uint64_t before = 0;
+            for (uint32_t s0 = 0; s0 < n; s0 += THREADS) {
+                if (n > THREADS) at = scan(p, s0, sh, q, mine, sum);
+                at += before;
+                if (at <= in_head && in_head < at + mine) sh.found = q, sh.found_at = at;
+                before += sum;
+                if (in_head < before) break;
+            }
+            __syncthreads();
+            q = sh.found, found_at = sh.found_at;
         }
-        __syncthreads();
-        c.seq = seq_at(p, sh.found);
+        c.seq = q;
         c.blocks = blocks_of<ROWS>(p, c.seq);
-        uint64_t rest = in_head - sh.found_at;
-        const uint32_t lane = threadIdx.x & 31;
+        uint64_t rest = in_head - found_at;
         for (uint32_t b0 = 0;; b0 += 32) {  // every warp for itself
             uint32_t first = 0, units = 0;
             if (b0 + lane < c.blocks) block_units<ROWS, UNIT>(p, c.seq, b0 + lane, first, units);
@@ -232,13 +259,18 @@ struct Line {
 };
 
 /// A part of an item in the workspace: ROWS rows of DP unnormalised sums, four columns of all rows after four of all rows, then
-/// the rows' maxima (in powers of two) and sums.
+/// the rows' maxima (in powers of two) and sums. The marks lie behind the parts.
 template <uint32_t ROWS, uint32_t DP>
 struct Part {
     static constexpr uint32_t FLOATS = ROWS * DP + 2 * ROWS, TOP = ROWS * DP, SUM = TOP + ROWS;
+    static constexpr uint64_t bytes(uint64_t parts) { return parts * 2 * (FLOATS * sizeof(float) + sizeof(uint64_t)); }
     /// `head`: the start of an item, else its middle or end.
     static __device__ __forceinline__ float *at(float *work, uint32_t part, bool head) { return work + ((size_t)part * 2 + head) * FLOATS; }
     static __device__ __forceinline__ uint32_t four(uint32_t row, uint32_t col4) { return (col4 * ROWS + row) * 4; }
+    static __device__ __forceinline__ uint64_t *mark(const Params &p, uint32_t part, bool head)
+    {
+        return reinterpret_cast<uint64_t *>(p.work + (size_t)p.parts * 2 * FLOATS) + (size_t)part * 2 + head;
+    }
 };
 
 __device__ __forceinline__ float exp2_fast(float x)
@@ -262,63 +294,74 @@ __device__ __forceinline__ void row_at(const Params &p, const Seq &q, uint32_t k
     token += q.row0;
 }
 
-/// Adds up the parts of the items that cuts divide: a block per cut and RP rows, the first cut in an item does it. A thread has
-/// one row and every (THREADS / RP)-th four columns of it.
-template <uint32_t ROWS, uint32_t UNIT, uint32_t DP, uint32_t RP>
-__global__ void __launch_bounds__(128) attn_paged_combine_kernel(const Params p)
+__device__ __forceinline__ void fence_gpu() { asm volatile("fence.sc.gpu;" ::: "memory"); }
+
+/// The end of a block: its parts, one of the item that it began in the middle of (pending[0]) and one of the item whose start it has
+/// (pending[1]), are marked and, where it is the last of an item's blocks to come, added up. All threads call this behind a barrier that
+/// follows the last store to the workspace.
+///
+/// The marks need no preparation: a mark is a number of this call's own, and a part of another call, or what the workspace held before,
+/// has another one. Each block writes its marks, then (behind a full fence) reads those of the others, so one of them sees all.
+/// More than one may: they write the same sums. Whoever has added up takes the marks away, for a replay of this call has the same number.
+template <uint32_t ROWS, uint32_t UNIT, uint32_t DP, uint32_t THREADS>
+__device__ void finish_parts(const Params &p, const Line<ROWS, UNIT, THREADS> &l, const Pending *pending, const bool (&has)[2])
 {
-    constexpr uint32_t THREADS = 128;
-    using L = Line<ROWS, UNIT, THREADS>;
     using P = Part<ROWS, DP>;
-    asm volatile("griddepcontrol.launch_dependents;");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    __shared__ typename L::Shared sh;
-    L l;
-    Cursor c;
-    uint64_t u;
-    const uint32_t part = blockIdx.x + 1;
-    if (!l.start(p, part, sh, u, c)) return;
-    const uint64_t from = u - c.u0, to = from + c.units;
-    if (c.u0 == 0 || l.cut(part - 1) > from) return;  // between two items; or an earlier cut is in this one
-    const uint32_t last = l.part_of(to - 1), rows = c.seq.news * p.group, d = p.cache.head_dim;
-    const uint32_t r = blockIdx.y * RP + threadIdx.x % RP, row = c.block * ROWS + r;
-    if (row >= rows) return;
-    auto at = [&](uint32_t k) { return P::at(p.work, k, k == part - 1); };
-    constexpr uint32_t NX = (DP / 4 + THREADS / RP - 1) / (THREADS / RP);  // fours of columns of a thread
-    const uint32_t x0 = threadIdx.x / RP;
-    // One pass over the parts, in the order of the keys, the sums scaled when the maximum grows: a part's loads are issued together.
-    float m = -INFINITY, sum = 0.0f;
-    float4 o[NX];
-#pragma unroll
-    for (uint32_t i = 0; i < NX; ++i) o[i] = make_float4(0, 0, 0, 0);
-#pragma unroll 2
-    for (uint32_t k = part - 1; k <= last; ++k) {
-        const float *a = at(k);
-        const float top = __ldcg(a + P::TOP + r), den = __ldcg(a + P::SUM + r);
-        float4 v[NX];
-#pragma unroll
-        for (uint32_t i = 0; i < NX; ++i) {
-            const uint32_t x = x0 + i * (THREADS / RP);
-            if (x * 4 < d) v[i] = __ldcg(reinterpret_cast<const float4 *>(a + P::four(r, x)));
-        }
-        const float all = fmaxf(m, top), ref = all == -INFINITY ? 0.0f : all;
-        const float f = exp2_fast(m - ref), g = exp2_fast(top - ref);
-        m = all;
-        sum = sum * f + den * g;
-#pragma unroll
-        for (uint32_t i = 0; i < NX; ++i) {
-            o[i].x = o[i].x * f + v[i].x * g, o[i].y = o[i].y * f + v[i].y * g;
-            o[i].z = o[i].z * f + v[i].z * g, o[i].w = o[i].w * f + v[i].w * g;
-        }
+    if (!has[0] && !has[1]) return;
+    const uint32_t tid = threadIdx.x, me = blockIdx.x, d = p.cache.head_dim;
+    if (tid == 0) {
+        fence_gpu();
+        for (uint32_t i = 0; i < 2; ++i)
+            if (has[i]) *(volatile uint64_t *)P::mark(p, me, i) = p.mark;
+        fence_gpu();
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    uint32_t token, head;
-    row_at(p, c.seq, c.kv_head, row, token, head);
-    uint16_t *out = p.out + ((size_t)token * p.n_heads + head) * d;
+    __syncthreads();
+    for (uint32_t i = 0; i < 2; ++i) {
+        if (!has[i]) continue;
+        const Pending &w = pending[i];
+        const uint32_t first = l.part_of(w.from), last = l.part_of(w.from + w.c.units - 1);
+        bool there = true;
+        for (uint32_t k = first + tid; k <= last; k += THREADS) there &= *(volatile uint64_t *)P::mark(p, k, k == first) == p.mark;
+        if (first + tid <= last) fence_gpu();
+        if (!__syncthreads_and(there)) continue;
+        // Four fours of columns of a row each: 32 bytes of the result, a sector.
+        const Seq &q = w.c.seq;
+        const uint32_t rows = min(q.news * p.group - w.c.block * ROWS, ROWS), wide = (d + 15) / 16;
+        for (uint32_t z = tid; z < ROWS * wide; z += THREADS) {
+            const uint32_t r = z % ROWS, x0 = z / ROWS * 4;
+            if (r >= rows) continue;
+            float m = -INFINITY, sum = 0.0f;
+            float4 o[4];
 #pragma unroll
-    for (uint32_t i = 0; i < NX; ++i) {
-        const uint32_t x = x0 + i * (THREADS / RP);
-        if (x * 4 < d) *reinterpret_cast<uint2 *>(out + x * 4) = make_uint2(bf16_pair(o[i].x * inv, o[i].y * inv), bf16_pair(o[i].z * inv, o[i].w * inv));
+            for (uint32_t y = 0; y < 4; ++y) o[y] = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+            for (uint32_t k = first; k <= last; ++k) {
+                const float *a = P::at(p.work, k, k == first);
+                const float top = __ldcg(a + P::TOP + r), den = __ldcg(a + P::SUM + r);
+                float4 v[4];
+#pragma unroll
+                for (uint32_t y = 0; y < 4; ++y)
+                    v[y] = (x0 + y) * 4 < d ? __ldcg(reinterpret_cast<const float4 *>(a + P::four(r, x0 + y))) : make_float4(0, 0, 0, 0);
+                const float all = fmaxf(m, top), ref = all == -INFINITY ? 0.0f : all;
+                const float f = exp2_fast(m - ref), g = exp2_fast(top - ref);
+                m = all;
+                sum = sum * f + den * g;
+#pragma unroll
+                for (uint32_t y = 0; y < 4; ++y) {
+                    o[y].x = o[y].x * f + v[y].x * g, o[y].y = o[y].y * f + v[y].y * g;
+                    o[y].z = o[y].z * f + v[y].z * g, o[y].w = o[y].w * f + v[y].w * g;
+                }
+            }
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            uint32_t token, head;
+            row_at(p, q, w.c.kv_head, w.c.block * ROWS + r, token, head);
+            uint16_t *out = p.out + ((size_t)token * p.n_heads + head) * d;
+#pragma unroll
+            for (uint32_t y = 0; y < 4; ++y)
+                if ((x0 + y) * 4 < d)
+                    *reinterpret_cast<uint2 *>(out + (x0 + y) * 4) = make_uint2(bf16_pair(o[y].x * inv, o[y].y * inv), bf16_pair(o[y].z * inv, o[y].w * inv));
+        }
+        for (uint32_t k = first + tid; k <= last; k += THREADS) *(volatile uint64_t *)P::mark(p, k, k == first) = 0;
     }
 }
 

@@ -2,12 +2,16 @@
 //
 // One pass over the keys with the running maximum and sum of the softmax. An item is 16 rows (the M of mma.sync m16n8k16) of
 // one sequence and key head; a part of its keys belongs to a block (attn_paged_common.cuh), whose warps take steps of 16 keys
-// in turn. A warp has its own ring of steps in shared memory, filled with cp.async 16 bytes at a time (rows of K and V at
-// swizzled chunks, keys that do not exist as zeros), its own maxima, sums and 16 x D accumulators in registers, so nothing but
-// its own copies makes it wait; the warps meet at the end of the item's part.
+// in turn. A warp has its own ring of tiles (16 keys of K, of V) in shared memory, its own maxima, sums and 16 x D accumulators in
+// registers, so nothing but its own copies makes it wait; the warps meet at the end of the item's part.
 //
-// The weights p of a step are rounded to bf16 for the product with V: relative 2^-9 each, independent, against the 2^-9 of the
-// output's own rounding; their sum is taken in f32 before that.
+// Tiles come by TMA, 64 columns wide with the 128-byte swizzle, which is also what ldmatrix reads without bank conflicts: a tile
+// is one or two copies per 64 columns where pages are a multiple of eight tokens. Other pages, by row, with cp.async. (Rows with
+// cp.async throughout: 32 address computations and copies per lane and step of 16 x 128, 4.7 TB/s over 130001 keys and 3.8 TB/s
+// of wide heads, where the instructions of four warps bounded it.)
+//
+// The weights p of a step are rounded to bf16 for the product with V: relative 2^-8 at most, each its own way, against the 2^-8 of
+// the output's own rounding; their sum is taken in f32 before that.
 //
 // Bound by memory: a step of 16 keys is 64 D bytes and D / 2 MMAs of 16 x 8 x 16.
 #pragma once
@@ -20,14 +24,20 @@ constexpr uint32_t kSplitRows = 16, kSplitUnit = 64, kStep = 16;
 
 template <int DP>
 struct SplitCfg {
-    static constexpr uint32_t WARPS = DP <= 128 ? 8 : 4, THREADS = WARPS * 32;
-    static constexpr uint32_t ROW = DP * 2, TILE = kStep * ROW, STAGE = 2 * TILE;  // bytes
-    static constexpr uint32_t STAGES = DP == 64 ? 6 : DP == 192 ? 4 : 3;
-    static constexpr uint32_t RING = STAGES * STAGE;
-    static constexpr uint32_t Q_BYTES = kSplitRows * ROW;
-    static constexpr uint32_t MASK_BYTES = WARPS * STAGES * 4, ML_BYTES = WARPS * kSplitRows * 8;
-    static constexpr uint32_t SMEM = WARPS * RING + Q_BYTES + MASK_BYTES + ML_BYTES;
+    static constexpr uint32_t WARPS = 8, THREADS = WARPS * 32;
+    static constexpr uint32_t CHUNKS = DP / 64;            // 64-column chunks of a row
+    static constexpr uint32_t CHUNK = kStep * 128, TILE = CHUNKS * CHUNK;  // bytes
+    static constexpr uint32_t SLOTS = 24576 / TILE;        // of a warp's ring: 12, 6, 4, 3
+    static constexpr uint32_t RING = SLOTS * TILE;
+    static constexpr uint32_t Q_BYTES = kSplitRows * DP * 2;
+    static constexpr uint32_t ML_BYTES = WARPS * kSplitRows * 8, BAR_BYTES = WARPS * SLOTS * 8;
+    static constexpr uint32_t SMEM = WARPS * RING + Q_BYTES + ML_BYTES + BAR_BYTES;
     static_assert(RING >= kSplitRows * DP * 4, "a warp's accumulators lie in its ring when warps meet");
+};
+
+struct SplitParams {
+    Params p;
+    uint32_t box;  // tokens per TMA box: 8 or 16
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool live)
@@ -40,6 +50,15 @@ __device__ __forceinline__ void cp_async_wait()
 {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+/// Box of the cache: 64 columns of one key head, some tokens of one page.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
+        "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4])
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
@@ -54,36 +73,51 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-/// Byte offset of 16-byte chunk c of row r in a tile with rows of DP bf16: chunks of eight rows fall on different banks.
-template <int DP>
-__device__ __forceinline__ uint32_t chunk_at(uint32_t r, uint32_t c)
-{
-    return r * (DP * 2) + ((c ^ (r & 7u)) << 4);
-}
+/// Byte offset of 16-byte piece c of row r of a tile of 16 rows: 64-column chunks one behind the other, 128-byte swizzle.
+__device__ __forceinline__ uint32_t piece_at(uint32_t r, uint32_t c) { return (c >> 3) * (kStep * 128) + r * 128 + (((c ^ r) & 7u) << 4); }
 
-template <int DP>
-__global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1) attn_paged_split_kernel(const Params p)
+template <int DP, bool TMA>
+__global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
+    attn_paged_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SplitParams sp)
 {
     using C = SplitCfg<DP>;
-    constexpr uint32_t ROWS = kSplitRows, UNIT = kSplitUnit;
+    using P = Part<kSplitRows, DP>;
+    constexpr uint32_t ROWS = kSplitRows, UNIT = kSplitUnit, SLOTS = C::SLOTS;
     asm volatile("griddepcontrol.launch_dependents;");
+    const Params &p = sp.p;
     extern __shared__ __align__(1024) uint8_t smem[];
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t ring = q4k::smem_u32(smem) + warp * C::RING;
-    const uint32_t q_smem = q4k::smem_u32(smem) + C::WARPS * C::RING;
-    uint32_t *masks = reinterpret_cast<uint32_t *>(smem + C::WARPS * C::RING + C::Q_BYTES) + warp * C::STAGES;
-    float2 *ml = reinterpret_cast<float2 *>(smem + C::WARPS * C::RING + C::Q_BYTES + C::MASK_BYTES);  // [warp][row]
-    const uint32_t d = p.cache.head_dim, chunks = d / 8;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-
     using L = Line<ROWS, UNIT, C::THREADS>;
     __shared__ typename L::Shared shared;
+    __shared__ Pending pending[2];
+    __shared__ int abort_flag;
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const uint32_t ring = q4k::smem_u32(smem) + warp * C::RING, q_smem = q4k::smem_u32(smem) + C::WARPS * C::RING;
+    float2 *ml = reinterpret_cast<float2 *>(smem + C::WARPS * C::RING + C::Q_BYTES);  // [warp][row]
+    const uint32_t bars = q_smem + C::Q_BYTES + C::ML_BYTES + warp * SLOTS * 8;
+    const uint32_t d = p.cache.head_dim, pieces = d / 8;
+    volatile int *abortp = &abort_flag;
+    if (tid == 0) abort_flag = 0;
+    if (TMA && lane == 0) {
+        for (uint32_t s = 0; s < SLOTS; ++s) q4k::mbar_init(bars + 8 * s, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (warp == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+        }
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (TMA) asm volatile("fence.proxy.async.global;" ::: "memory");  // ordinary stores of the launch in front, read by the copy engine
+
     L line;
     Cursor cur;
     uint64_t u;
     if (!line.start(p, blockIdx.x, shared, u, cur)) return;
     const uint64_t u_end = line.cut(blockIdx.x + 1);
     if (u >= u_end) return;
+    bool has[2] = {cur.u0 > 0, false};
+    if (tid == 0) pending[0] = Pending{cur, u - cur.u0};
+    uint32_t at = 0, phases = 0;  // the ring's next slot, the parity of each slot's next phase
 
     while (true) {
         const uint32_t n_units = (uint32_t)min((uint64_t)(cur.units - cur.u0), u_end - u);
@@ -96,55 +130,96 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1) attn_paged_split_ker
         const uint32_t key0 = max((cur.first + u0) * UNIT, lo / kStep * kStep), key1 = min((cur.first + u0 + n_units) * UNIT, hi);
         const uint32_t steps = key1 > key0 ? (key1 - key0 + kStep - 1) / kStep : 0;
         const uint32_t mine = steps > warp ? (steps - warp + C::WARPS - 1) / C::WARPS : 0;
+        auto key_of = [&](uint32_t j) { return key0 + (warp + j * C::WARPS) * kStep; };
+
+        const int32_t *table = p.seqs.table + (size_t)seq.index * p.seqs.max_pages;
+        const uint32_t boxes = TMA ? kStep / sp.box : kStep, span = TMA ? sp.box : 1;
+        // Where the tokens of a step lie. TMA: lane l < boxes has the page of box l. Rows: lane l % 16 that of a row, as an offset.
+        struct Where {
+            uint32_t page, slot;  // page = num_pages: there is none
+        };
+        auto find = [&](uint32_t j) {
+            Where w{p.cache.num_pages, 0};
+            const uint32_t l = TMA ? lane : lane & 15u, key = key_of(j) + l * span;
+            if (j < mine && l < boxes && key < (TMA ? seq.keys : key1)) {
+                const uint32_t page = (uint32_t)__ldcg(table + key / p.cache.page_size);
+                if (page < p.cache.num_pages) w.page = page, w.slot = key % p.cache.page_size;
+            }
+            return w;
+        };
+        // The tile of K or V of a step into slot `to`.
+        auto request = [&](const Where &w, bool v, uint32_t to) {
+            const uint32_t dst = ring + to * C::TILE;
+            if constexpr (TMA) {
+                if (lane == 0) q4k::mbar_expect_tx(bars + 8 * to, C::TILE);
+                __syncwarp();
+                if (lane < boxes) {
+#pragma unroll
+                    for (uint32_t c = 0; c < C::CHUNKS; ++c)
+                        tma_load_4d(dst + c * C::CHUNK + lane * sp.box * 128, v ? &map_v : &map_k, (int)(c * 64), (int)kv_head, (int)w.slot, (int)w.page,
+                                    bars + 8 * to);
+                }
+            } else {
+                const uint16_t *base = v ? p.cache.v : p.cache.k;
+#pragma unroll 4
+                for (uint32_t c = lane; c < kStep * (DP / 8); c += 32) {
+                    const uint32_t r = c / (DP / 8), cc = c % (DP / 8);
+                    const uint32_t page = __shfl_sync(0xffffffffu, w.page, r), slot = __shfl_sync(0xffffffffu, w.slot, r);
+                    const bool ok = page < p.cache.num_pages && cc < pieces;
+                    const size_t off = page * p.cache.page_stride + (uint64_t)slot * p.cache.token_stride + (uint64_t)kv_head * p.cache.head_stride + cc * 8;
+                    cp_async16(dst + piece_at(r, cc), base + (ok ? off : 0), ok);
+                }
+                cp_async_commit();
+            }
+        };
+        // Tiles K_0, V_0, K_1, ... of this warp. In flight: SLOTS of them. `holes`: for each of the steps that are on their way, the boxes
+        // (or a row: any) that are not there, two bits at step % 16.
+        uint32_t holes = 0;
+        bool row_hole = false;  // rows: some row of some step is not there
+        auto note = [&](uint32_t j, const Where &w) {
+            if constexpr (TMA) {
+                const uint32_t gone = __ballot_sync(0xffffffffu, lane < boxes && w.page >= p.cache.num_pages);
+                holes = (holes & ~(3u << (j % 16 * 2))) | (gone << (j % 16 * 2));
+            } else {
+                row_hole |= __any_sync(0xffffffffu, w.page >= p.cache.num_pages && j < mine);
+            }
+        };
+        constexpr uint32_t H = SLOTS / 2;
+        constexpr bool ODD = SLOTS % 2;
+        Where ahead{0, 0};  // of step j + H: whose K, and V, are requested next; ODD: of the step whose V is
+#pragma unroll
+        for (uint32_t j = 0; j < H + ODD; ++j) {
+            const Where w = find(j);
+            note(j, w);
+            const uint32_t k_to = (at + 2 * j) % SLOTS, v_to = (at + 2 * j + 1) % SLOTS;
+            if (j < mine) request(w, false, k_to);
+            else if (!TMA) cp_async_commit();
+            if (j < H) {
+                if (j < mine) request(w, true, v_to);
+                else if (!TMA) cp_async_commit();
+            }
+            ahead = w;
+        }
+        Where next = find(H + ODD);
+        if (!ODD) ahead = next;
 
         // Q rows, zeros past the last row and column.
         for (uint32_t c = tid; c < ROWS * (DP / 8); c += C::THREADS) {
             const uint32_t r = c / (DP / 8), cc = c % (DP / 8);
             uint4 v = make_uint4(0, 0, 0, 0);
-            if (row0 + r < rows && cc < chunks) {
+            if (row0 + r < rows && cc < pieces) {
                 uint32_t token, head;
                 row_at(p, seq, kv_head, row0 + r, token, head);
                 v = __ldcg(reinterpret_cast<const uint4 *>(p.q + (size_t)token * p.q_stride + (size_t)head * d + cc * 8));
             }
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(q_smem + chunk_at<DP>(r, cc)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(q_smem + piece_at(r, cc)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
         }
-
-        const int32_t *table = p.seqs.table + (size_t)seq.index * p.seqs.max_pages;
-        const size_t head_off = (size_t)kv_head * p.cache.head_stride;
-        // Lane l of a warp knows where key l % 16 of a step lies: -1 where there is none.
-        auto locate = [&](uint32_t j) -> int64_t {
-            const uint32_t key = key0 + (warp + j * C::WARPS) * kStep + (lane & 15u);
-            if (j >= mine || key >= key1) return -1;
-            const uint32_t page = (uint32_t)__ldcg(table + key / p.cache.page_size);
-            if (page >= p.cache.num_pages) return -1;
-            return (int64_t)(page * p.cache.page_stride + (uint64_t)(key % p.cache.page_size) * p.cache.token_stride + head_off);
-        };
-        auto request = [&](uint32_t j, int64_t at) {  // step j of this warp into stage j % STAGES
-            const uint32_t stage = j % C::STAGES, dst = ring + stage * C::STAGE;
-            const uint32_t live = __ballot_sync(0xffffffffu, at >= 0) & 0xffffu;
-            if (lane == 0) masks[stage] = live;
-#pragma unroll 4
-            for (uint32_t c = lane; c < kStep * (DP / 8); c += 32) {
-                const uint32_t r = c / (DP / 8), cc = c % (DP / 8);
-                const int64_t row = __shfl_sync(0xffffffffu, at, r);
-                const bool ok = row >= 0 && cc < chunks;
-                const size_t off = ok ? (size_t)row + cc * 8 : 0;
-                cp_async16(dst + chunk_at<DP>(r, cc), p.cache.k + off, ok);
-                cp_async16(dst + C::TILE + chunk_at<DP>(r, cc), p.cache.v + off, ok);
-            }
-        };
-#pragma unroll
-        for (uint32_t j = 0; j < C::STAGES - 1; ++j) {
-            if (j < mine) request(j, locate(j));
-            cp_async_commit();
-        }
-        int64_t next = locate(C::STAGES - 1);
         __syncthreads();  // Q is there
 
         constexpr bool Q_REGS = DP <= 128;
         uint32_t qf[Q_REGS ? DP / 16 : 1][4];
         // A of k-slice k: rows lane % 16, columns 16 k + 8 (lane / 16)
-        auto q_frag = [&](uint32_t k, uint32_t (&f)[4]) { ldsm4(q_smem + chunk_at<DP>(lane & 15u, 2 * k + (lane >> 4)), f); };
+        auto q_frag = [&](uint32_t k, uint32_t (&f)[4]) { ldsm4(q_smem + piece_at(lane & 15u, 2 * k + (lane >> 4)), f); };
         if constexpr (Q_REGS) {
 #pragma unroll
             for (uint32_t k = 0; k < DP / 16; ++k) q_frag(k, qf[k]);
@@ -157,8 +232,7 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1) attn_paged_split_ker
         uint32_t lo_r[2], hi_r[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t r = row0 + lane / 4 + 8 * h;
-            const uint32_t i = min(r, rows - 1) / p.group;
+            const uint32_t i = min(row0 + lane / 4 + 8 * h, rows - 1) / p.group;
             key_range(p, seq, i, i, lo_r[h], hi_r[h]);
         }
         uint32_t lo_all, hi_all;  // what every row of the block sees
@@ -167,17 +241,37 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1) attn_paged_split_ker
             key_range(p, seq, i1, i1, lo_all, t);
             key_range(p, seq, i0, i0, t, hi_all);
         }
-
+        // The next tile in the ring has arrived: its slot.
+        auto arrived = [&](uint32_t &slot) {
+            slot = at;
+            bool ok = true;
+            if constexpr (TMA) {
+                ok = __all_sync(0xffffffffu, q4k::mbar_wait(bars + 8 * at, (phases >> at) & 1u, abortp));
+                phases ^= 1u << at;
+                if (!ok && lane == 0) *(volatile uint32_t *)p.status = (32u << 24) | blockIdx.x;
+            } else {
+                cp_async_wait<SLOTS - 1>();
+                __syncwarp();
+            }
+            if (++at == SLOTS) at = 0;
+            return ok;
+        };
+        uint32_t done = 0;  // tiles that have arrived
         for (uint32_t j = 0; j < mine; ++j) {
-            cp_async_wait<C::STAGES - 2>();
-            __syncwarp();
-            const uint32_t stage = j % C::STAGES, kt = ring + stage * C::STAGE, vt = kt + C::TILE;
-            const uint32_t key = key0 + (warp + j * C::WARPS) * kStep, live = masks[stage];
-            if (j + C::STAGES - 1 < mine) request(j + C::STAGES - 1, next);
-            cp_async_commit();
-            next = locate(j + C::STAGES);
-
+            const uint32_t key = key_of(j);
+            uint32_t kt, vt;
+            if (!arrived(kt)) break;
+            ++done;
+            uint32_t gone = 0;  // bit t: key t is not there
+            if constexpr (TMA) {
+                const uint32_t b = (holes >> (j % 16 * 2)) & 3u;
+                gone = sp.box == 8 ? (b & 1u ? 0xffu : 0u) | (b & 2u ? 0xff00u : 0u) : b ? 0xffffu : 0u;
+            } else if (row_hole) {
+                const uint32_t k = key + (lane & 15u);
+                gone = __ballot_sync(0xffffffffu, k < key1 && (uint32_t)__ldcg(table + k / p.cache.page_size) >= p.cache.num_pages) & 0xffffu;
+            }
             float sc[2][4] = {};
+            const uint32_t ka = ring + kt * C::TILE;
 #pragma unroll
             for (uint32_t k = 0; k < DP / 16; ++k) {
                 uint32_t a[4], b[4];
@@ -188,21 +282,32 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1) attn_paged_split_ker
                     q_frag(k, a);
                 }
                 // keys 0-7 then 8-15, columns 16 k and 8 more
-                ldsm4(kt + chunk_at<DP>((lane & 7u) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1u)), b);
+                ldsm4(ka + piece_at((lane & 7u) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1u)), b);
                 mma_bf16(sc[0], a, b[0], b[1]);
                 mma_bf16(sc[1], a, b[2], b[3]);
+            }
+            __syncwarp();  // the tile is read
+            if (ODD) {
+                if (j + H < mine) request(ahead, true, kt);
+                else if (!TMA) cp_async_commit();
+                ahead = next;
+                next = find(j + H + 2);
+            } else {
+                if (j + H < mine) note(j + H, ahead), request(ahead, false, kt);
+                else if (!TMA) cp_async_commit();
+                next = find(j + H + 1);
             }
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) sc[n][x] *= p.scale_log2;
-            if (live != 0xffffu || key < lo_all || key + kStep > hi_all) {
+            if (gone || key < lo_all || key + kStep > min(hi_all, key1)) {
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         const uint32_t t = 8 * n + 2 * (lane & 3u) + (x & 1);
-                        if (!((live >> t) & 1u) || key + t < lo_r[x >> 1] || key + t >= hi_r[x >> 1]) sc[n][x] = -INFINITY;
+                        if (((gone >> t) & 1u) || key + t < lo_r[x >> 1] || key + t >= min(hi_r[x >> 1], key1)) sc[n][x] = -INFINITY;
                     }
             }
             float scale_o[2];
@@ -229,17 +334,47 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1) attn_paged_split_ker
                 for (uint32_t n = 0; n < DP / 8; ++n) o[n][0] *= scale_o[0], o[n][1] *= scale_o[0], o[n][2] *= scale_o[1], o[n][3] *= scale_o[1];
             }
             const uint32_t pf[4] = {bf16_pair(sc[0][0], sc[0][1]), bf16_pair(sc[0][2], sc[0][3]), bf16_pair(sc[1][0], sc[1][1]), bf16_pair(sc[1][2], sc[1][3])};
+            if (!arrived(vt)) break;
+            ++done;
+            const uint32_t va = ring + vt * C::TILE;
+            if (TMA && key + kStep > seq.keys) {  // slots behind the sequence may hold anything: no values
+                const uint32_t first = seq.keys - key;
+                for (uint32_t c = lane + first * (DP / 8); c < kStep * (DP / 8); c += 32)
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(va + piece_at(c / (DP / 8), c % (DP / 8))), "r"(0) : "memory");
+                fence_async_smem();  // the slot's next writer is the copy engine
+                __syncwarp();
+            }
 #pragma unroll
             for (uint32_t n = 0; n < DP / 16; ++n) {
                 uint32_t b[4];
                 // keys 0-7, 8-15 of columns 16 n, then of 8 more
-                ldsm4_t(vt + chunk_at<DP>(lane & 15u, 2 * n + (lane >> 4)), b);
+                ldsm4_t(va + piece_at(lane & 15u, 2 * n + (lane >> 4)), b);
                 mma_bf16(o[2 * n], pf, b[0], b[1]);
                 mma_bf16(o[2 * n + 1], pf, b[2], b[3]);
             }
-            __syncwarp();  // the stage is read
+            __syncwarp();  // the tile is read
+            if (ODD) {
+                if (j + H + 1 < mine) note(j + H + 1, ahead), request(ahead, false, vt);
+                else if (!TMA) cp_async_commit();
+            } else {
+                if (j + H < mine) request(ahead, true, vt);
+                else if (!TMA) cp_async_commit();
+                ahead = next;
+            }
         }
-        cp_async_wait<0>();
+        if constexpr (TMA) {
+            if (*abortp && done < 2 * mine) {  // what is on its way must land before the block ends
+                const uint32_t on_way = min(2 * mine - done, SLOTS);
+                const long long t0 = clock64();
+                for (uint32_t k = 0; k < on_way; ++k) {
+                    const uint32_t slot = (at + k) % SLOTS;
+                    while (!q4k::mbar_try(bars + 8 * slot, (phases >> slot) & 1u))
+                        if (clock64() - t0 > 20000000ll) break;
+                }
+            }
+        } else {
+            cp_async_wait<0>();
+        }
 
         // ---- the warps meet: sums to the block's maximum, every warp's accumulators in its ring ----
 #pragma unroll
@@ -249,23 +384,21 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1) attn_paged_split_ker
             if ((lane & 3u) == 0) ml[warp * ROWS + lane / 4 + 8 * h] = make_float2(m[h], l[h]);
         }
         __syncthreads();
-        float top[2];
+        if (*abortp) return;  // of the whole block: no thread sets it between the barriers
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             float t = -INFINITY;
 #pragma unroll
             for (uint32_t w = 0; w < C::WARPS; ++w) t = fmaxf(t, ml[w * ROWS + lane / 4 + 8 * h].x);
-            top[h] = t;
             const float f = m[h] == -INFINITY ? 0.0f : exp2_fast(m[h] - t);
             float *dst = reinterpret_cast<float *>(smem + warp * C::RING) + (lane / 4 + 8 * h) * DP;
 #pragma unroll
-            for (uint32_t n = 0; n < DP / 8; ++n)  // 16-byte chunks swizzled: eight rows on different banks
+            for (uint32_t n = 0; n < DP / 8; ++n)  // 16-byte pieces swizzled: eight rows on different banks
                 *reinterpret_cast<float2 *>(dst + (((2 * n + ((lane >> 1) & 1u)) ^ (lane / 4)) << 2) + (lane & 1u) * 2) =
                     make_float2(o[n][2 * h] * f, o[n][2 * h + 1] * f);
         }
         __syncthreads();
         const bool whole = n_units == cur.units;
-        using P = Part<ROWS, DP>;
         float *part = P::at(p.work, blockIdx.x, u0 == 0);
         for (uint32_t c = tid; c < ROWS * (DP / 4); c += C::THREADS) {
             const uint32_t r = c / (DP / 4), x = c % (DP / 4);
@@ -294,11 +427,18 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1) attn_paged_split_ker
                 if (x == 0) part[P::TOP + r] = t, part[P::SUM + r] = den;
             }
         }
+        if (!whole && u0 == 0) {
+            has[1] = true;
+            if (tid == 0) pending[1] = Pending{cur, u};
+        }
         u += n_units;
-        if (u >= u_end) return;
+        if (u >= u_end) break;
         L::next(p, cur);
-        __syncthreads();  // rings, Q and ml are read
+        if (TMA) fence_async_smem();  // the rings' next writer is the copy engine
+        __syncthreads();              // rings, Q and ml are read
     }
+    __syncthreads();
+    finish_parts<ROWS, UNIT, DP, C::THREADS>(p, line, pending, has);
 }
 
 }  // namespace attn

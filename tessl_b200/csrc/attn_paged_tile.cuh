@@ -21,7 +21,7 @@
 // Roles: eight warps softmax, Q and the results, one warp TMA, a warp for each row tile MMA issue. Every wait is bounded; on a
 // timeout the status word is set and all roles fall through to the end.
 #pragma once
-#include "attn_paged_common.cuh"
+#include "attn_paged_split.cuh"
 #include "prefill_common.cuh"
 
 namespace tessl {
@@ -46,7 +46,7 @@ struct TileCfg {
     static constexpr uint32_t SLOTS = DP == 64 ? 11 : DP == 192 ? 3 : 5;
     static constexpr uint32_t BARS_T = 3 * NS + 2, NBARS = 2 * SLOTS + NT * BARS_T + 1;
     static constexpr uint32_t X_BYTES = TPR == 2 ? NS * 2 * 128 * 4 : 0;  // what the two threads of a row tell each other
-    static constexpr uint32_t SMEM = Q_BYTES + SLOTS * SLOT + X_BYTES + NBARS * 8 + 16;
+    static constexpr uint32_t SMEM = Q_BYTES + SLOTS * SLOT + X_BYTES + NBARS * 8 + 2 * sizeof(Pending) + 16;
     static constexpr uint32_t TMA_WARP = 4 * NT * TPR, MMA_WARP = TMA_WARP + 1, THREADS = (MMA_WARP + NT) * 32;
     static constexpr uint32_t S_COL = 256;                 // TMEM columns: accumulators from 0, scores from here
     static_assert(SMEM <= 227 * 1024, "shared memory");    // none of it static: the dynamic part starts at a multiple of 1 KiB
@@ -60,14 +60,6 @@ struct TileParams {
     uint32_t negate;   // the scale is negative: the first product's A operand is negated instead
 };
 
-/// Box of the cache: 64 columns of one key head, `box` tokens of one page.
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar)
-{
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
-        "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
-        : "memory");
-}
 // A converged warp issues the MMAs, one election for four of them: descriptors stay warp-uniform values. (From a branch of one lane
 // 16 MMAs took ~1500 clocks to issue, three times as long as to run.)
 /// D[tmem] (+)= A[smem] . B[smem]^T, K = 64: two 64-column chunks, K-major, by the low words of their descriptors.
@@ -158,7 +150,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
         : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ uint64_t f32_pair(float lo, float hi)
 {
     uint64_t r;
@@ -204,6 +195,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
     const uint32_t q_smem = q4k::smem_u32(smem_raw), ring = q_smem + C::Q_BYTES, bar0 = ring + C::SLOTS * C::SLOT + C::X_BYTES;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem_raw + C::SMEM - 16);
     volatile int *abortp = reinterpret_cast<volatile int *>(smem_raw + C::SMEM - 8);
+    Pending *pending = reinterpret_cast<Pending *>(smem_raw + C::SMEM - 16 - 2 * sizeof(Pending));  // items of which this block has a part
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     auto slot_full = [&](uint32_t s) { return bar0 + 8 * s; };
     auto slot_empty = [&](uint32_t s) { return bar0 + 8 * (C::SLOTS + s); };
@@ -247,7 +239,14 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
     L line;
     Cursor cur;
     uint64_t u = 0, u_end = 0;
+    bool has[2] = {false, false};
     if (line.start(p, blockIdx.x, *reinterpret_cast<typename L::Shared *>(smem_raw + C::Q_BYTES), u, cur)) u_end = line.cut(blockIdx.x + 1);
+    const uint64_t u_start = u;
+    if (tid == 0) pending[1].from = ~0ull;
+    if (u < u_end) {
+        has[0] = cur.u0 > 0;
+        if (tid == 0) pending[0] = Pending{cur, u - cur.u0};
+    }
     fence_async_smem();  // the ring's next writer is the copy engine
     __syncthreads();
     // The item at the cursor, as every role sees it: n tiles of keys from k0 on, in `steps` steps.
@@ -591,6 +590,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                 }
             }
             const bool whole = n_units == cur.units;
+            if (!whole && cur.u0 == 0 && tid == 0) pending[1] = Pending{cur, u};
             float *part = P::at(p.work, blockIdx.x, cur.u0 == 0);
             tiles += 2 * n;
             u += n_units;
@@ -666,6 +666,9 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
         pf::tcgen05_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(pf::kTmemCols) : "memory");
     }
+    if (*abortp || u_start >= u_end) return;
+    has[1] = pending[1].from != ~0ull;
+    finish_parts<C::ROWS, kTileKeys, DP, C::THREADS>(p, line, pending, has);
 }
 
 }  // namespace attn
