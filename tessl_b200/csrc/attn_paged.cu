@@ -65,7 +65,6 @@ Result launch_split(TesslRuntime *rt, const Params &p)
     const char *what = "attn_paged launch";
     attn::SplitParams sp{p, box_of(p.cache.page_size, attn::kStep)};
     sp.p.parts = (uint32_t)rt->sm_count;
-    sp.p.min_units = 2;
     CUtensorMap map_k{}, map_v{};
     auto go = [&](auto kernel) -> Result {
         TESSL_TRY(smem_opt_in(rt, (const void *)kernel, C::SMEM, what, true));
@@ -85,13 +84,12 @@ Result launch_tiles(TesslRuntime *rt, const Params &p, bool negate)
     TESSL_TRY(smem_opt_in(rt, (const void *)kernel, C::SMEM, what, true));
     attn::TileParams tp{p, box_of(p.cache.page_size, attn::kTileKeys), negate};
     tp.p.parts = (uint32_t)rt->sm_count;
-    tp.p.min_units = 4;
     CUtensorMap map_k, map_v;
     TESSL_TRY(cache_maps(rt, what, p.cache, tp.box, &map_k, &map_v));
     return launch_pdl(rt, what, kernel, dim3(tp.p.parts), dim3(C::THREADS), C::SMEM, map_k, map_v, tp);
 }
 
-/// A number that no other call's parts are marked with: the n-th of a sequence that differs from runtime to runtime (splitmix64).
+/// A number of 48 bits that no other call's items are counted with: the n-th of a sequence that differs from runtime to runtime (splitmix64).
 uint64_t next_mark(TesslRuntime *rt)
 {
     if (!rt->attn_mark) {
@@ -101,8 +99,8 @@ uint64_t next_mark(TesslRuntime *rt)
     uint64_t z = rt->attn_mark += 0x9e3779b97f4a7c15ull;
     z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
     z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
-    z ^= z >> 31;
-    return z ? z : 1;  // 0 is no mark
+    z = (z ^ (z >> 31)) >> 16;
+    return z ? z : 1;  // 0 is nobody's
 }
 
 Result attn_params(const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t n_heads, const char *what, Params *p)
@@ -113,6 +111,9 @@ Result attn_params(const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32
         return fmt("%s: n_heads %u is not a multiple of n_kv_heads %u", what, n_heads, cache.n_kv_heads);
     TESSL_TRY(require_i32_extent(elems(total_new, n_heads), "attn_paged: total_new * n_heads"));
     p->n_heads = n_heads, p->group = n_heads / cache.n_kv_heads;
+    p->page_shift = 32;
+    for (uint32_t b = 0; b < 32; ++b)
+        if (cache.page_size == 1u << b) p->page_shift = b;
     return ok();
 }
 

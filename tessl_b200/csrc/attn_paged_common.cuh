@@ -6,9 +6,9 @@
 // call, item after item, are one line that is cut into equal parts, one per block of the launch: whatever the lengths of the
 // sequences, every block reads the same number of keys. The lengths are on the device, so the blocks work the cuts out
 // themselves. A block that has an item to itself writes its rows; the parts of an item that a cut divides go to the workspace,
-// two at most per block (the end of one item, the start of another). A block marks its parts when it is done and looks whether those
-// of the others are marked: the last one to come adds them up, in the order of the keys, the same sums on every run. (A second
-// launch for the sums took 9 us of the 18 of a token over 777 keys, and 21 of 74 of ragged chunks.)
+// two at most per block (the end of one item, the start of another). A block counts its parts in when it is done: the last one of an
+// item to come adds the parts up, in the order of the keys, the same sums on every run. (A second launch for the sums took 9 us
+// of the 18 of a token over 777 keys, and 21 of 74 of ragged chunks.)
 #pragma once
 #include "paged_common.cuh"
 #include "q4_gemv_tma.cuh"
@@ -25,11 +25,18 @@ struct Params {
     uint32_t q_stride, n_heads, group;
     float scale_log2;  // scale * log2 e
     uint32_t causal, window;
+    uint32_t page_shift;  // log2 of a page size that is a power of two, else 32
     uint32_t parts;      // blocks that the line of units may be cut for
-    uint32_t min_units;  // units that a part is worth
-    uint64_t mark;       // of this call's parts
+    uint64_t mark;       // of this call's items: 48 bits
     uint32_t *status;
 };
+
+/// Page and slot of a token of a sequence.
+__device__ __forceinline__ uint32_t page_index(const Params &p, uint32_t key) { return p.page_shift < 32 ? key >> p.page_shift : key / p.cache.page_size; }
+__device__ __forceinline__ uint32_t page_slot(const Params &p, uint32_t key)
+{
+    return p.page_shift < 32 ? key & (p.cache.page_size - 1) : key % p.cache.page_size;
+}
 
 /// One sequence as its rows see it.
 struct Seq {
@@ -89,84 +96,109 @@ struct Pending {
     uint64_t from;
 };
 
-/// The line of units (key heads, in each the sequences, in each the blocks of rows) and how it is cut.
-template <uint32_t ROWS, uint32_t UNIT, uint32_t THREADS>
+/// The line of the call's work (key heads, in each the sequences, in each the blocks of rows) and how it is cut: its units, or, where
+/// cutting items would cost more than it gives, whole items. EXTRA: what an item's second part costs, in units.
+template <uint32_t ROWS, uint32_t UNIT, uint32_t THREADS, uint32_t EXTRA>
 struct Line {
+    /// Of some sequences, for one key head.
+    struct Count {
+        uint64_t units;
+        uint32_t blocks, most;  // most: units of one block
+        __device__ __forceinline__ void add(uint64_t u, uint32_t b, uint32_t m) { units += u, blocks += b, most = max(most, m); }
+    };
     struct Shared {
-        uint64_t warp_sum[THREADS / 32], cost[THREADS];
+        Count warp_sum[THREADS / 32], cost[THREADS];
         uint32_t many[THREADS], n_many;
         uint64_t found_at;
         Seq found;
     };
-    uint64_t per_head, total;
-    uint32_t parts;
+    uint64_t per_head, each;
+    uint32_t parts, longer;  // the first `longer` parts have each + 1
+    bool whole;              // items are not cut: the line counts items
 
-    __device__ __forceinline__ uint64_t cut(uint32_t c) const { return total / parts * c + total % parts * c / parts; }
-    /// The part that holds unit u.
+    /// a / b; sums of units seldom leave 32 bits.
+    static __device__ __forceinline__ uint64_t div(uint64_t a, uint64_t b)
+    {
+        if ((a | b) >> 32 == 0) return (uint32_t)a / (uint32_t)b;
+        return a / b;
+    }
+    __device__ __forceinline__ uint64_t cut(uint32_t c) const { return each * c + min(c, longer); }
+    /// The part that holds place u.
     __device__ __forceinline__ uint32_t part_of(uint64_t u) const
     {
-        uint32_t c = (uint32_t)min((uint64_t)parts - 1, (uint64_t)((double)u / (double)total * parts));
-        while (c > 0 && cut(c) > u) --c;
-        while (c + 1 < parts && cut(c + 1) <= u) ++c;
+        const uint64_t edge = (each + 1) * longer;
+        return u < edge ? (uint32_t)div(u, each + 1) : longer + (uint32_t)div(u - edge, each);
+    }
+    /// Units of the item at the cursor that lie between places u and u_end, and how far they reach.
+    __device__ __forceinline__ uint32_t units_to(const Cursor &c, uint64_t u, uint64_t u_end) const
+    {
+        return whole ? c.units : (uint32_t)min((uint64_t)(c.units - c.u0), u_end - u);
+    }
+    __device__ __forceinline__ uint64_t places(uint32_t units) const { return whole ? 1 : units; }
+
+    /// Every `step`-th block of a sequence from b0 on.
+    static __device__ __forceinline__ Count count(const Params &p, const Seq &q, uint32_t blocks, uint32_t b0, uint32_t step)
+    {
+        Count c{0, 0, 0};
+        for (uint32_t b = b0; b < blocks; b += step) {
+            uint32_t first, units;
+            block_units<ROWS, UNIT>(p, q, b, first, units);
+            c.add(units, 1, units);
+        }
+        return c;
+    }
+    static __device__ __forceinline__ Count warp_total(Count c)
+    {
+#pragma unroll
+        for (uint32_t o = 16; o > 0; o /= 2)
+            c.add(__shfl_xor_sync(0xffffffffu, c.units, o), __shfl_xor_sync(0xffffffffu, c.blocks, o), __shfl_xor_sync(0xffffffffu, c.most, o));
         return c;
     }
 
-    /// Units in front of this thread's sequence s0 + threadIdx.x among those of the block, its own in `mine`, all in `sum`.
+    /// Counts this thread's sequence s0 + threadIdx.x: what lies in front of it among those of the block, itself (`mine`), all (`sum`).
     /// Sequences of many blocks of rows are counted by a warp each.
-    static __device__ uint64_t scan(const Params &p, uint32_t s0, Shared &sh, Seq &q, uint64_t &mine, uint64_t &sum)
+    static __device__ Count scan(const Params &p, uint32_t s0, Shared &sh, Seq &q, Count &mine, Count &sum)
     {
         const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = s0 + tid;
         __syncthreads();  // sh may still be read
         if (tid == 0) sh.n_many = 0;
         __syncthreads();
-        uint64_t cost = 0;
+        mine = Count{0, 0, 0};
+        bool many = false;
         if (s < p.seqs.num_seqs) {
             q = seq_at(p, s);
             const uint32_t blocks = blocks_of<ROWS>(p, q);
-            if (blocks > 2) {
-                sh.many[atomicAdd(&sh.n_many, 1u)] = tid;
-            } else {
-                for (uint32_t b = 0; b < blocks; ++b) {
-                    uint32_t first, units;
-                    block_units<ROWS, UNIT>(p, q, b, first, units);
-                    cost += units;
-                }
-            }
+            many = blocks > 2;
+            if (many) sh.many[atomicAdd(&sh.n_many, 1u)] = tid;
+            else mine = count(p, q, blocks, 0, 1);
         }
-        sh.cost[tid] = cost;
         __syncthreads();
         for (uint32_t i = warp; i < sh.n_many; i += THREADS / 32) {
-            const uint32_t t = sh.many[i];
-            const Seq r = seq_at(p, s0 + t);
-            const uint32_t blocks = blocks_of<ROWS>(p, r);
-            uint64_t c = 0;
-            for (uint32_t b = lane; b < blocks; b += 32) {
-                uint32_t first, units;
-                block_units<ROWS, UNIT>(p, r, b, first, units);
-                c += units;
-            }
-#pragma unroll
-            for (uint32_t o = 16; o > 0; o /= 2) c += __shfl_xor_sync(0xffffffffu, c, o);
-            if (lane == 0) sh.cost[t] = c;
+            const Seq r = seq_at(p, s0 + sh.many[i]);
+            const Count c = warp_total(count(p, r, blocks_of<ROWS>(p, r), lane, 32));
+            if (lane == 0) sh.cost[sh.many[i]] = c;
         }
         if (sh.n_many) __syncthreads();
-        mine = sh.cost[tid];
-        uint64_t run = mine;
+        if (many) mine = sh.cost[tid];
+        Count run = mine;
 #pragma unroll
         for (uint32_t o = 1; o < 32; o *= 2) {
-            const uint64_t t = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += t;
+            const uint64_t t = __shfl_up_sync(0xffffffffu, run.units, o);
+            const uint32_t b = __shfl_up_sync(0xffffffffu, run.blocks, o), m = __shfl_up_sync(0xffffffffu, run.most, o);
+            if (lane >= o) run.add(t, b, m);
         }
         if (lane == 31) sh.warp_sum[warp] = run;
         __syncthreads();
-        uint64_t before = 0;
-        sum = 0;
+        Count before{0, 0, 0};
+        sum = before;
 #pragma unroll
         for (uint32_t w = 0; w < THREADS / 32; ++w) {
-            if (w < warp) before += sh.warp_sum[w];
-            sum += sh.warp_sum[w];
+            const Count &t = sh.warp_sum[w];
+            if (w < warp) before.add(t.units, t.blocks, 0);
+            sum.add(t.units, t.blocks, t.most);
         }
-        return before + run - mine;
+        before.add(run.units - mine.units, run.blocks - mine.blocks, 0);
+        return before;
     }
 
     /// The whole block calls this, and has one of: no part (false), or in `from` its place in the line and the item there. The
@@ -174,43 +206,41 @@ struct Line {
     __device__ bool start(const Params &p, uint32_t part, Shared &sh, uint64_t &from, Cursor &c)
     {
         const uint32_t n = p.seqs.num_seqs, lane = threadIdx.x & 31;
-        uint64_t mine, sum, at, found_at = 0;
+        Count mine, sum, all, at;
+        uint64_t found_at = 0;
         Seq q;
         if (n == 1) {  // every warp for itself
             q = seq_at(p, 0);
             const uint32_t blocks = blocks_of<ROWS>(p, q);
-            sum = 0;
-            for (uint32_t b = lane; b < blocks; b += 32) {
-                uint32_t first, units;
-                block_units<ROWS, UNIT>(p, q, b, first, units);
-                sum += units;
-            }
-#pragma unroll
-            for (uint32_t o = 16; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            per_head = sum;
+            all = blocks == 1 ? count(p, q, 1, 0, 1) : warp_total(count(p, q, blocks, lane, 32));
         } else {
             at = scan(p, 0, sh, q, mine, sum);
-            per_head = sum;
+            all = sum;
             for (uint32_t s0 = THREADS; s0 < n; s0 += THREADS) {
-                uint64_t m, t;
+                Count m, t;
                 Seq other;
                 scan(p, s0, sh, other, m, t);
-                per_head += t;
+                all.add(t.units, t.blocks, t.most);
             }
         }
-        total = per_head * p.cache.n_kv_heads;
-        parts = (uint32_t)min((uint64_t)p.parts, max((uint64_t)1, total / p.min_units));
-        if (part >= parts || total == 0) return false;
+        // The longest part: units cut evenly and an item's second part, or as many of the largest items as a part has items.
+        const uint64_t items = (uint64_t)all.blocks * p.cache.n_kv_heads, units = all.units * p.cache.n_kv_heads;
+        whole = (div(items + p.parts - 1, p.parts)) * all.most <= div(units, p.parts) + EXTRA;
+        const uint64_t total = whole ? items : units;
+        per_head = whole ? all.blocks : all.units;
+        parts = (uint32_t)min((uint64_t)p.parts, total);
+        if (part >= parts) return false;
+        each = div(total, parts), longer = (uint32_t)(total - each * parts);
         from = cut(part);
-        const uint64_t in_head = from % per_head;
-        c.kv_head = (uint32_t)(from / per_head);
+        c.kv_head = (uint32_t)div(from, per_head);
+        const uint64_t in_head = from - c.kv_head * per_head;
         if (n > 1) {
             uint64_t before = 0;
             for (uint32_t s0 = 0; s0 < n; s0 += THREADS) {
                 if (n > THREADS) at = scan(p, s0, sh, q, mine, sum);
-                at += before;
-                if (at <= in_head && in_head < at + mine) sh.found = q, sh.found_at = at;
-                before += sum;
+                const uint64_t place = before + (whole ? at.blocks : at.units);
+                if (place <= in_head && in_head < place + (whole ? mine.blocks : mine.units)) sh.found = q, sh.found_at = place;
+                before += whole ? sum.blocks : sum.units;
                 if (in_head < before) break;
             }
             __syncthreads();
@@ -219,6 +249,11 @@ struct Line {
         c.seq = q;
         c.blocks = blocks_of<ROWS>(p, c.seq);
         uint64_t rest = in_head - found_at;
+        if (whole || c.blocks == 1) {
+            c.block = whole ? (uint32_t)rest : 0, c.u0 = whole ? 0 : (uint32_t)rest;
+            block_units<ROWS, UNIT>(p, c.seq, c.block, c.first, c.units);
+            return true;
+        }
         for (uint32_t b0 = 0;; b0 += 32) {  // every warp for itself
             uint32_t first = 0, units = 0;
             if (b0 + lane < c.blocks) block_units<ROWS, UNIT>(p, c.seq, b0 + lane, first, units);
@@ -259,17 +294,17 @@ struct Line {
 };
 
 /// A part of an item in the workspace: ROWS rows of DP unnormalised sums, four columns of all rows after four of all rows, then
-/// the rows' maxima (in powers of two) and sums. The marks lie behind the parts.
+/// the rows' maxima (in powers of two) and sums. Behind the parts a counter for each block: of the item whose start it has.
 template <uint32_t ROWS, uint32_t DP>
 struct Part {
     static constexpr uint32_t FLOATS = ROWS * DP + 2 * ROWS, TOP = ROWS * DP, SUM = TOP + ROWS;
-    static constexpr uint64_t bytes(uint64_t parts) { return parts * 2 * (FLOATS * sizeof(float) + sizeof(uint64_t)); }
+    static constexpr uint64_t bytes(uint64_t parts) { return parts * (2 * FLOATS * sizeof(float) + sizeof(uint64_t)); }
     /// `head`: the start of an item, else its middle or end.
     static __device__ __forceinline__ float *at(float *work, uint32_t part, bool head) { return work + ((size_t)part * 2 + head) * FLOATS; }
     static __device__ __forceinline__ uint32_t four(uint32_t row, uint32_t col4) { return (col4 * ROWS + row) * 4; }
-    static __device__ __forceinline__ uint64_t *mark(const Params &p, uint32_t part, bool head)
+    static __device__ __forceinline__ unsigned long long *counter(const Params &p, uint32_t part)
     {
-        return reinterpret_cast<uint64_t *>(p.work + (size_t)p.parts * 2 * FLOATS) + (size_t)part * 2 + head;
+        return reinterpret_cast<unsigned long long *>(p.work + (size_t)p.parts * 2 * FLOATS) + part;
     }
 };
 
@@ -294,40 +329,40 @@ __device__ __forceinline__ void row_at(const Params &p, const Seq &q, uint32_t k
     token += q.row0;
 }
 
-__device__ __forceinline__ void fence_gpu() { asm volatile("fence.sc.gpu;" ::: "memory"); }
-
 /// The end of a block: its parts, one of the item that it began in the middle of (pending[0]) and one of the item whose start it has
-/// (pending[1]), are marked and, where it is the last of an item's blocks to come, added up. All threads call this behind a barrier that
-/// follows the last store to the workspace.
+/// (pending[1]), are counted in and, where it is the last of an item's blocks to come, added up. All threads call this behind a
+/// barrier that follows the last store to the workspace; `came`: two words of shared memory.
 ///
-/// The marks need no preparation: a mark is a number of this call's own, and a part of another call, or what the workspace held before,
-/// has another one. Each block writes its marks, then (behind a full fence) reads those of the others, so one of them sees all.
-/// More than one may: they write the same sums. Whoever has added up takes the marks away, for a replay of this call has the same number.
-template <uint32_t ROWS, uint32_t UNIT, uint32_t DP, uint32_t THREADS>
-__device__ void finish_parts(const Params &p, const Line<ROWS, UNIT, THREADS> &l, const Pending *pending, const bool (&has)[2])
+/// The counters need no preparation. One holds a number of this call's own and a count; what another call or nobody has put there
+/// has another number and stands for a count of 0. Whoever has added up puts a 0 there, for a replay of this call has the same number.
+template <uint32_t DP, uint32_t ROWS, typename L>
+__device__ void finish_parts(const Params &p, const L &l, const Pending *pending, const bool (&has)[2], uint32_t threads,
+                             volatile uint32_t *came)
 {
     using P = Part<ROWS, DP>;
     if (!has[0] && !has[1]) return;
-    const uint32_t tid = threadIdx.x, me = blockIdx.x, d = p.cache.head_dim;
-    if (tid == 0) {
-        fence_gpu();
-        for (uint32_t i = 0; i < 2; ++i)
-            if (has[i]) *(volatile uint64_t *)P::mark(p, me, i) = p.mark;
-        fence_gpu();
+    const uint32_t tid = threadIdx.x, d = p.cache.head_dim;
+    if (tid < 2 && has[tid]) {
+        __threadfence();  // the block's parts, behind the barrier that all have passed
+        unsigned long long *const at = P::counter(p, l.part_of(pending[tid].from));
+        unsigned long long seen = 0, old;
+        do {
+            old = seen;
+            seen = atomicCAS(at, old, (old >> 16 == p.mark ? old : p.mark << 16) + 1);
+        } while (seen != old);
+        came[tid] = (uint32_t)(old >> 16 == p.mark ? old & 0xffffu : 0) + 1;
+        __threadfence();
     }
     __syncthreads();
     for (uint32_t i = 0; i < 2; ++i) {
         if (!has[i]) continue;
         const Pending &w = pending[i];
         const uint32_t first = l.part_of(w.from), last = l.part_of(w.from + w.c.units - 1);
-        bool there = true;
-        for (uint32_t k = first + tid; k <= last; k += THREADS) there &= *(volatile uint64_t *)P::mark(p, k, k == first) == p.mark;
-        if (first + tid <= last) fence_gpu();
-        if (!__syncthreads_and(there)) continue;
+        if (came[i] != last - first + 1) continue;
         // Four fours of columns of a row each: 32 bytes of the result, a sector.
         const Seq &q = w.c.seq;
         const uint32_t rows = min(q.news * p.group - w.c.block * ROWS, ROWS), wide = (d + 15) / 16;
-        for (uint32_t z = tid; z < ROWS * wide; z += THREADS) {
+        for (uint32_t z = tid; z < ROWS * wide; z += threads) {
             const uint32_t r = z % ROWS, x0 = z / ROWS * 4;
             if (r >= rows) continue;
             float m = -INFINITY, sum = 0.0f;
@@ -361,7 +396,7 @@ __device__ void finish_parts(const Params &p, const Line<ROWS, UNIT, THREADS> &l
                 if ((x0 + y) * 4 < d)
                     *reinterpret_cast<uint2 *>(out + (x0 + y) * 4) = make_uint2(bf16_pair(o[y].x * inv, o[y].y * inv), bf16_pair(o[y].z * inv, o[y].w * inv));
         }
-        for (uint32_t k = first + tid; k <= last; k += THREADS) *(volatile uint64_t *)P::mark(p, k, k == first) = 0;
+        if (tid == 0) *P::counter(p, first) = 0;
     }
 }
 

@@ -21,6 +21,7 @@ namespace tessl {
 namespace attn {
 
 constexpr uint32_t kSplitRows = 16, kSplitUnit = 64, kStep = 16;
+constexpr uint32_t kSplitExtra = 16;  // a second part costs as much as 1024 keys
 
 template <int DP>
 struct SplitCfg {
@@ -86,10 +87,11 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
     asm volatile("griddepcontrol.launch_dependents;");
     const Params &p = sp.p;
     extern __shared__ __align__(1024) uint8_t smem[];
-    using L = Line<ROWS, UNIT, C::THREADS>;
+    using L = Line<ROWS, UNIT, C::THREADS, kSplitExtra>;
     __shared__ typename L::Shared shared;
     __shared__ Pending pending[2];
     __shared__ int abort_flag;
+    __shared__ uint32_t came[2];
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t ring = q4k::smem_u32(smem) + warp * C::RING, q_smem = q4k::smem_u32(smem) + C::WARPS * C::RING;
     float2 *ml = reinterpret_cast<float2 *>(smem + C::WARPS * C::RING + C::Q_BYTES);  // [warp][row]
@@ -120,7 +122,7 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
     uint32_t at = 0, phases = 0;  // the ring's next slot, the parity of each slot's next phase
 
     while (true) {
-        const uint32_t n_units = (uint32_t)min((uint64_t)(cur.units - cur.u0), u_end - u);
+        const uint32_t n_units = line.units_to(cur, u, u_end);
         const Seq &seq = cur.seq;
         const uint32_t kv_head = cur.kv_head, u0 = cur.u0, rows = seq.news * p.group, row0 = cur.block * ROWS;
         // Keys of this part that the block's rows may see.
@@ -142,8 +144,8 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
             Where w{p.cache.num_pages, 0};
             const uint32_t l = TMA ? lane : lane & 15u, key = key_of(j) + l * span;
             if (j < mine && l < boxes && key < (TMA ? seq.keys : key1)) {
-                const uint32_t page = (uint32_t)__ldcg(table + key / p.cache.page_size);
-                if (page < p.cache.num_pages) w.page = page, w.slot = key % p.cache.page_size;
+                const uint32_t page = (uint32_t)__ldcg(table + page_index(p, key));
+                if (page < p.cache.num_pages) w.page = page, w.slot = page_slot(p, key);
             }
             return w;
         };
@@ -186,22 +188,20 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
         };
         constexpr uint32_t H = SLOTS / 2;
         constexpr bool ODD = SLOTS % 2;
-        Where ahead{0, 0};  // of step j + H: whose K, and V, are requested next; ODD: of the step whose V is
+        Where first[H + ODD + 1];  // looked up together
+#pragma unroll
+        for (uint32_t j = 0; j < H + ODD + 1; ++j) first[j] = find(j);
 #pragma unroll
         for (uint32_t j = 0; j < H + ODD; ++j) {
-            const Where w = find(j);
-            note(j, w);
-            const uint32_t k_to = (at + 2 * j) % SLOTS, v_to = (at + 2 * j + 1) % SLOTS;
-            if (j < mine) request(w, false, k_to);
+            note(j, first[j]);
+            if (j < mine) request(first[j], false, (at + 2 * j) % SLOTS);
             else if (!TMA) cp_async_commit();
             if (j < H) {
-                if (j < mine) request(w, true, v_to);
+                if (j < mine) request(first[j], true, (at + 2 * j + 1) % SLOTS);
                 else if (!TMA) cp_async_commit();
             }
-            ahead = w;
         }
-        Where next = find(H + ODD);
-        if (!ODD) ahead = next;
+        Where ahead = first[H], next = first[H + ODD];  // of step j + H: whose K, and V, are requested next; ODD: of the step whose V is
 
         // Q rows, zeros past the last row and column.
         for (uint32_t c = tid; c < ROWS * (DP / 8); c += C::THREADS) {
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
                 gone = sp.box == 8 ? (b & 1u ? 0xffu : 0u) | (b & 2u ? 0xff00u : 0u) : b ? 0xffffu : 0u;
             } else if (row_hole) {
                 const uint32_t k = key + (lane & 15u);
-                gone = __ballot_sync(0xffffffffu, k < key1 && (uint32_t)__ldcg(table + k / p.cache.page_size) >= p.cache.num_pages) & 0xffffu;
+                gone = __ballot_sync(0xffffffffu, k < key1 && (uint32_t)__ldcg(table + page_index(p, k)) >= p.cache.num_pages) & 0xffffu;
             }
             float sc[2][4] = {};
             const uint32_t ka = ring + kt * C::TILE;
@@ -400,9 +400,9 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
         __syncthreads();
         const bool whole = n_units == cur.units;
         float *part = P::at(p.work, blockIdx.x, u0 == 0);
-        for (uint32_t c = tid; c < ROWS * (DP / 4); c += C::THREADS) {
+        for (uint32_t c = tid; c < min(ROWS, rows - row0) * (DP / 4); c += C::THREADS) {
             const uint32_t r = c / (DP / 4), x = c % (DP / 4);
-            if (row0 + r >= rows || x * 4 >= d) continue;
+            if (x * 4 >= d) continue;
             float4 sum = make_float4(0, 0, 0, 0);
             float t = -INFINITY, den = 0.0f;
 #pragma unroll
@@ -431,14 +431,14 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
             has[1] = true;
             if (tid == 0) pending[1] = Pending{cur, u};
         }
-        u += n_units;
+        u += line.places(n_units);
         if (u >= u_end) break;
         L::next(p, cur);
         if (TMA) fence_async_smem();  // the rings' next writer is the copy engine
         __syncthreads();              // rings, Q and ml are read
     }
     __syncthreads();
-    finish_parts<ROWS, UNIT, DP, C::THREADS>(p, line, pending, has);
+    finish_parts<DP, ROWS>(p, line, pending, has, C::THREADS, came);
 }
 
 }  // namespace attn

@@ -28,6 +28,7 @@ namespace tessl {
 namespace attn {
 
 constexpr uint32_t kTileKeys = 128;
+constexpr uint32_t kTileExtra = 6;  // a second part of an item costs as much as six tiles of keys
 
 template <int DP>
 struct TileCfg {
@@ -46,11 +47,11 @@ struct TileCfg {
     static constexpr uint32_t SLOTS = DP == 64 ? 11 : DP == 192 ? 3 : 5;
     static constexpr uint32_t BARS_T = 3 * NS + 2, NBARS = 2 * SLOTS + NT * BARS_T + 1;
     static constexpr uint32_t X_BYTES = TPR == 2 ? NS * 2 * 128 * 4 : 0;  // what the two threads of a row tell each other
-    static constexpr uint32_t SMEM = Q_BYTES + SLOTS * SLOT + X_BYTES + NBARS * 8 + 2 * sizeof(Pending) + 16;
+    static constexpr uint32_t SMEM = Q_BYTES + SLOTS * SLOT + X_BYTES + NBARS * 8 + 2 * sizeof(Pending) + 32;
     static constexpr uint32_t TMA_WARP = 4 * NT * TPR, MMA_WARP = TMA_WARP + 1, THREADS = (MMA_WARP + NT) * 32;
     static constexpr uint32_t S_COL = 256;                 // TMEM columns: accumulators from 0, scores from here
     static_assert(SMEM <= 227 * 1024, "shared memory");    // none of it static: the dynamic part starts at a multiple of 1 KiB
-    static_assert(sizeof(typename Line<ROWS, kTileKeys, THREADS>::Shared) <= SLOTS * SLOT, "the scan of the line uses the ring");
+    static_assert(sizeof(typename Line<ROWS, kTileKeys, THREADS, kTileExtra>::Shared) <= SLOTS * SLOT, "the scan of the line uses the ring");
     static_assert(SMEM > 227 * 1024 / 2, "two blocks on an SM would both want all of its TMEM");
 };
 
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
     attn_paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TileParams tp)
 {
     using C = TileCfg<DP>;
-    using L = Line<C::ROWS, kTileKeys, C::THREADS>;
+    using L = Line<C::ROWS, kTileKeys, C::THREADS, kTileExtra>;
     using P = Part<C::ROWS, DP>;
     using q4k::mbar_arrive;
     using q4k::mbar_expect_tx;
@@ -193,9 +194,9 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
     const Params &p = tp.p;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t q_smem = q4k::smem_u32(smem_raw), ring = q_smem + C::Q_BYTES, bar0 = ring + C::SLOTS * C::SLOT + C::X_BYTES;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem_raw + C::SMEM - 16);
-    volatile int *abortp = reinterpret_cast<volatile int *>(smem_raw + C::SMEM - 8);
-    Pending *pending = reinterpret_cast<Pending *>(smem_raw + C::SMEM - 16 - 2 * sizeof(Pending));  // items of which this block has a part
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem_raw + C::SMEM - 32);
+    volatile int *abortp = reinterpret_cast<volatile int *>(smem_raw + C::SMEM - 24);
+    Pending *pending = reinterpret_cast<Pending *>(smem_raw + C::SMEM - 32 - 2 * sizeof(Pending));  // items of which this block has a part
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     auto slot_full = [&](uint32_t s) { return bar0 + 8 * s; };
     auto slot_empty = [&](uint32_t s) { return bar0 + 8 * (C::SLOTS + s); };
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
     // The item at the cursor, as every role sees it: n tiles of keys from k0 on, in `steps` steps.
     uint32_t n_units, n, steps, k0, row0, rows;
     auto item = [&] {
-        n_units = (uint32_t)min((uint64_t)(cur.units - cur.u0), u_end - u);
+        n_units = line.units_to(cur, u, u_end);
         rows = cur.seq.news * p.group, row0 = cur.block * C::ROWS;
         uint32_t lo, hi;
         key_range(p, cur.seq, row0 / p.group, (min(row0 + C::ROWS, rows) - 1) / p.group, lo, hi);
@@ -298,8 +299,8 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                 const uint32_t key = k0 + j * kTileKeys + lane * tp.box;
                 page = (int)p.cache.num_pages, slot = 0;
                 if (j < n && lane < boxes && key < cur.seq.keys) {
-                    const uint32_t pg = (uint32_t)__ldcg(table + key / p.cache.page_size);
-                    if (pg < p.cache.num_pages) page = (int)pg, slot = (int)(key % p.cache.page_size);
+                    const uint32_t pg = (uint32_t)__ldcg(table + page_index(p, key));
+                    if (pg < p.cache.num_pages) page = (int)pg, slot = (int)page_slot(p, key);
                 }
             };
             constexpr uint32_t A = C::AHEAD;
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                 for (uint32_t i = 0; i < A; ++i) pk[i] = pk[i + 1], sk[i] = sk[i + 1];
                 pk[A] = np, sk[A] = ns;
             }
-            u += n_units;
+            u += line.places(n_units);
             if (u < u_end) L::next(p, cur);
         }
         if (*abortp && lane == 0) {  // what is on its way must land before the block ends
@@ -411,7 +412,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                         if (lane == 0) mbar_arrive(slot_empty(k_slot[s]));
             }
             tiles += 2 * n;
-            u += n_units;
+            u += line.places(n_units);
             if (u < u_end) L::next(p, cur);
         }
         // Also after an abort: nothing may still read shared memory or TMEM when the block ends.
@@ -499,7 +500,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                 }
                 const uint32_t lo_all = __shfl_sync(0xffffffffu, lo_r, 31), hi_all = __shfl_sync(0xffffffffu, hi_r, 0);
                 const int32_t *table = p.seqs.table + (size_t)cur.seq.index * p.seqs.max_pages;
-                auto page_of = [&](uint32_t key) { return key < cur.seq.keys ? (uint32_t)__ldcg(table + key / p.cache.page_size) : 0u; };
+                auto page_of = [&](uint32_t key) { return key < cur.seq.keys ? (uint32_t)__ldcg(table + page_index(p, key)) : 0u; };
                 bool any_hole = false;  // a page of the item is not there: its tiles look at theirs
                 for (uint32_t key = k0 + lane * tp.box; key < k0 + n * kTileKeys; key += 32 * tp.box) any_hole |= page_of(key) >= p.cache.num_pages;
                 any_hole = __any_sync(0xffffffffu, any_hole);
@@ -593,7 +594,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
             if (!whole && cur.u0 == 0 && tid == 0) pending[1] = Pending{cur, u};
             float *part = P::at(p.work, blockIdx.x, cur.u0 == 0);
             tiles += 2 * n;
-            u += n_units;
+            u += line.places(n_units);
             if (u < u_end) L::next(p, cur), item();
             load_q();  // of the next item, while the last product runs
             if (mine && n_steps) {
@@ -668,7 +669,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
     }
     if (*abortp || u_start >= u_end) return;
     has[1] = pending[1].from != ~0ull;
-    finish_parts<C::ROWS, kTileKeys, DP, C::THREADS>(p, line, pending, has);
+    finish_parts<DP, C::ROWS>(p, line, pending, has, C::THREADS, reinterpret_cast<volatile uint32_t *>(smem_raw + C::SMEM - 16));
 }
 
 }  // namespace attn

@@ -68,7 +68,7 @@ struct TesslRuntime {
     // The same for the split kernel: CTAs per tile (0 = not that kernel, -1 = the library decides).
     int prefill_force_split = -1;
     int prefill_last_split = 0;
-    // Marks of the parts that attention calls leave in their workspaces (0: none given out yet).
+    // Of the numbers that attention calls count their items in with (0: none given out yet).
     uint64_t attn_mark = 0;
     // Clock budget of a bounded device-side wait on another rank (0 = the default).
     uint64_t peer_wait_clocks = 0;
