@@ -110,10 +110,7 @@ Result attn_params(const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32
     if (n_heads == 0 || n_heads % cache.n_kv_heads != 0)
         return fmt("%s: n_heads %u is not a multiple of n_kv_heads %u", what, n_heads, cache.n_kv_heads);
     TESSL_TRY(require_i32_extent(elems(total_new, n_heads), "attn_paged: total_new * n_heads"));
-    p->n_heads = n_heads, p->group = n_heads / cache.n_kv_heads;
-    p->page_shift = 32;
-    for (uint32_t b = 0; b < 32; ++b)
-        if (cache.page_size == 1u << b) p->page_shift = b;
+    p->n_heads = n_heads, p->group = attn::Divisor::of(n_heads / cache.n_kv_heads), p->page = attn::Divisor::of(cache.page_size);
     return ok();
 }
 
@@ -144,7 +141,10 @@ Result attn_paged(TesslRuntime *rt, const TesslBuf &q, const TesslPagedKv &cache
     TESSL_TRY(require_aligned16(q, "attn_paged q"));
     TESSL_TRY(require_aligned16(out, "attn_paged out"));
     if (q_stride % 8 != 0) return fmt("%s: rows of q are %u apart, not a multiple of 8", what, q_stride);
-    const uint64_t need = workspace_of(rt, cache, seqs, total_new, p.group);
+    // The kernels count 16 rows x 64 keys at a time, in 32 bits.
+    const double blocks = (double)elems(total_new, p.group.d) / 16 + seqs.num_seqs, most = (double)std::min<uint64_t>(p.seqs.capacity, 0x7fffffffu) / 64 + 1;
+    if (blocks * most * cache.n_kv_heads >= 4294967296.0) return fmt("%s: more rows and keys than one call counts", what);
+    const uint64_t need = workspace_of(rt, cache, seqs, total_new, p.group.d);
     if (workspace.nbytes < need) return fmt("%s: the workspace has %llu bytes, the call needs %llu", what, (unsigned long long)workspace.nbytes, (unsigned long long)need);
     TESSL_TRY(require_aligned16(workspace, "attn_paged workspace"));
     if (!workspace.ptr) return fmt("%s: null workspace", what);
@@ -159,7 +159,7 @@ Result attn_paged(TesslRuntime *rt, const TesslBuf &q, const TesslPagedKv &cache
     p.scale_log2 = scale * 1.4426950408889634f;
     p.mark = next_mark(rt);
     // A scale of zero makes zeros of scores that a mask has set to -inf: the tile kernel masks before it scales.
-    const bool tiles = wants_tiles(cache, seqs, total_new, p.group) && p.scale_log2 != 0.0f;
+    const bool tiles = wants_tiles(cache, seqs, total_new, p.group.d) && p.scale_log2 != 0.0f;
     return with_dim(cache.head_dim, [&](auto dp) {
         constexpr int DP = decltype(dp)::value;
         if (!tiles) return launch_split<DP>(rt, p);

@@ -16,27 +16,40 @@
 namespace tessl {
 namespace attn {
 
+/// Division by a number that is the same for a whole launch, exact for every 32-bit dividend: the multiplication by a rounded-up
+/// reciprocal of Granlund and Montgomery. (The compiler's division is some thirty instructions, and what a block does once it runs from
+/// a cold instruction cache.)
+struct Divisor {
+    uint32_t d, m, s1, s2;
+    static Divisor of(uint32_t d)  // d >= 1
+    {
+        uint32_t l = 0;
+        while (l < 32 && (uint64_t(1) << l) < d) ++l;
+        return Divisor{d, (uint32_t)(((uint64_t(1) << 32) * ((uint64_t(1) << l) - d)) / d + 1), l < 1 ? l : 1, l > 0 ? l - 1 : 0};
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t x) const
+    {
+        const uint32_t t = __umulhi(m, x);
+        return (t + ((x - t) >> s1)) >> s2;
+    }
+    __device__ __forceinline__ uint32_t mod(uint32_t x) const { return x - div(x) * d; }
+};
+
 struct Params {
     const uint16_t *q;
     uint16_t *out;
     float *work;
     paged::Cache cache;
     paged::Seqs seqs;
-    uint32_t q_stride, n_heads, group;
+    uint32_t q_stride, n_heads;
+    Divisor group;  // query heads of a key head
+    Divisor page;   // tokens
     float scale_log2;  // scale * log2 e
     uint32_t causal, window;
-    uint32_t page_shift;  // log2 of a page size that is a power of two, else 32
     uint32_t parts;      // blocks that the line of units may be cut for
     uint64_t mark;       // of this call's items: 48 bits
     uint32_t *status;
 };
-
-/// Page and slot of a token of a sequence.
-__device__ __forceinline__ uint32_t page_index(const Params &p, uint32_t key) { return p.page_shift < 32 ? key >> p.page_shift : key / p.cache.page_size; }
-__device__ __forceinline__ uint32_t page_slot(const Params &p, uint32_t key)
-{
-    return p.page_shift < 32 ? key & (p.cache.page_size - 1) : key % p.cache.page_size;
-}
 
 /// One sequence as its rows see it.
 struct Seq {
@@ -73,16 +86,16 @@ __device__ __forceinline__ void key_range(const Params &p, const Seq &q, uint32_
 template <uint32_t ROWS, uint32_t UNIT>
 __device__ __forceinline__ void block_units(const Params &p, const Seq &q, uint32_t block, uint32_t &first, uint32_t &units)
 {
-    const uint32_t rows = q.news * p.group, r0 = block * ROWS;
+    const uint32_t rows = q.news * p.group.d, r0 = block * ROWS;
     uint32_t lo, hi;
-    key_range(p, q, r0 / p.group, (min(r0 + ROWS, rows) - 1) / p.group, lo, hi);
+    key_range(p, q, p.group.div(r0), p.group.div(min(r0 + ROWS, rows) - 1), lo, hi);
     first = lo / UNIT;
     units = max(1u, (hi + UNIT - 1) / UNIT - first);
 }
 template <uint32_t ROWS>
 __device__ __forceinline__ uint32_t blocks_of(const Params &p, const Seq &q)
 {
-    return (q.news * p.group + ROWS - 1) / ROWS;
+    return (q.news * p.group.d + ROWS - 1) / ROWS;
 }
 
 /// An item, and where in it a part begins.
@@ -93,48 +106,40 @@ struct Cursor {
 /// An item of which a block has a part, and where the item begins on the line.
 struct Pending {
     Cursor c;
-    uint64_t from;
+    uint32_t from;
 };
 
 /// The line of the call's work (key heads, in each the sequences, in each the blocks of rows) and how it is cut: its units, or, where
 /// cutting items would cost more than it gives, whole items. EXTRA: what an item's second part costs, in units.
 template <uint32_t ROWS, uint32_t UNIT, uint32_t THREADS, uint32_t EXTRA>
 struct Line {
-    /// Of some sequences, for one key head.
+    /// Of some sequences, for one key head. The host has made sure that a call's units are below 2^32.
     struct Count {
-        uint64_t units;
-        uint32_t blocks, most;  // most: units of one block
-        __device__ __forceinline__ void add(uint64_t u, uint32_t b, uint32_t m) { units += u, blocks += b, most = max(most, m); }
+        uint32_t units, blocks, most;  // most: units of one block
+        __device__ __forceinline__ void add(uint32_t u, uint32_t b, uint32_t m) { units += u, blocks += b, most = max(most, m); }
     };
     struct Shared {
         Count warp_sum[THREADS / 32], cost[THREADS];
-        uint32_t many[THREADS], n_many;
-        uint64_t found_at;
+        uint32_t many[THREADS], n_many, found_at;
         Seq found;
     };
-    uint64_t per_head, each;
+    uint32_t per_head, each;
     uint32_t parts, longer;  // the first `longer` parts have each + 1
     bool whole;              // items are not cut: the line counts items
 
-    /// a / b; sums of units seldom leave 32 bits.
-    static __device__ __forceinline__ uint64_t div(uint64_t a, uint64_t b)
-    {
-        if ((a | b) >> 32 == 0) return (uint32_t)a / (uint32_t)b;
-        return a / b;
-    }
-    __device__ __forceinline__ uint64_t cut(uint32_t c) const { return each * c + min(c, longer); }
+    __device__ __forceinline__ uint32_t cut(uint32_t c) const { return each * c + min(c, longer); }
     /// The part that holds place u.
-    __device__ __forceinline__ uint32_t part_of(uint64_t u) const
+    __device__ __forceinline__ uint32_t part_of(uint32_t u) const
     {
-        const uint64_t edge = (each + 1) * longer;
-        return u < edge ? (uint32_t)div(u, each + 1) : longer + (uint32_t)div(u - edge, each);
+        const uint32_t edge = (each + 1) * longer;
+        return u < edge ? u / (each + 1) : longer + (u - edge) / each;
     }
     /// Units of the item at the cursor that lie between places u and u_end, and how far they reach.
-    __device__ __forceinline__ uint32_t units_to(const Cursor &c, uint64_t u, uint64_t u_end) const
+    __device__ __forceinline__ uint32_t units_to(const Cursor &c, uint32_t u, uint32_t u_end) const
     {
-        return whole ? c.units : (uint32_t)min((uint64_t)(c.units - c.u0), u_end - u);
+        return whole ? c.units : min(c.units - c.u0, u_end - u);
     }
-    __device__ __forceinline__ uint64_t places(uint32_t units) const { return whole ? 1 : units; }
+    __device__ __forceinline__ uint32_t places(uint32_t units) const { return whole ? 1 : units; }
 
     /// Every `step`-th block of a sequence from b0 on.
     static __device__ __forceinline__ Count count(const Params &p, const Seq &q, uint32_t blocks, uint32_t b0, uint32_t step)
@@ -183,8 +188,7 @@ struct Line {
         Count run = mine;
 #pragma unroll
         for (uint32_t o = 1; o < 32; o *= 2) {
-            const uint64_t t = __shfl_up_sync(0xffffffffu, run.units, o);
-            const uint32_t b = __shfl_up_sync(0xffffffffu, run.blocks, o), m = __shfl_up_sync(0xffffffffu, run.most, o);
+            const uint32_t t = __shfl_up_sync(0xffffffffu, run.units, o), b = __shfl_up_sync(0xffffffffu, run.blocks, o), m = __shfl_up_sync(0xffffffffu, run.most, o);
             if (lane >= o) run.add(t, b, m);
         }
         if (lane == 31) sh.warp_sum[warp] = run;
@@ -203,11 +207,11 @@ struct Line {
 
     /// The whole block calls this, and has one of: no part (false), or in `from` its place in the line and the item there. The
     /// sequences are gone over twice where a block's threads do not hold them all.
-    __device__ bool start(const Params &p, uint32_t part, Shared &sh, uint64_t &from, Cursor &c)
+    __device__ bool start(const Params &p, uint32_t part, Shared &sh, uint32_t &from, Cursor &c)
     {
         const uint32_t n = p.seqs.num_seqs, lane = threadIdx.x & 31;
         Count mine, sum, all, at;
-        uint64_t found_at = 0;
+        uint32_t found_at = 0;
         Seq q;
         if (n == 1) {  // every warp for itself
             q = seq_at(p, 0);
@@ -224,21 +228,21 @@ struct Line {
             }
         }
         // The longest part: units cut evenly and an item's second part, or as many of the largest items as a part has items.
-        const uint64_t items = (uint64_t)all.blocks * p.cache.n_kv_heads, units = all.units * p.cache.n_kv_heads;
-        whole = (div(items + p.parts - 1, p.parts)) * all.most <= div(units, p.parts) + EXTRA;
-        const uint64_t total = whole ? items : units;
+        const uint32_t items = all.blocks * p.cache.n_kv_heads, units = all.units * p.cache.n_kv_heads;
+        whole = (items + p.parts - 1) / p.parts * (uint64_t)all.most <= units / p.parts + EXTRA;
+        const uint32_t total = whole ? items : units;
         per_head = whole ? all.blocks : all.units;
-        parts = (uint32_t)min((uint64_t)p.parts, total);
+        parts = min(p.parts, total);
         if (part >= parts) return false;
-        each = div(total, parts), longer = (uint32_t)(total - each * parts);
+        each = total / parts, longer = total - each * parts;
         from = cut(part);
-        c.kv_head = (uint32_t)div(from, per_head);
-        const uint64_t in_head = from - c.kv_head * per_head;
+        c.kv_head = from / per_head;
+        const uint32_t in_head = from - c.kv_head * per_head;
         if (n > 1) {
-            uint64_t before = 0;
+            uint32_t before = 0;
             for (uint32_t s0 = 0; s0 < n; s0 += THREADS) {
                 if (n > THREADS) at = scan(p, s0, sh, q, mine, sum);
-                const uint64_t place = before + (whole ? at.blocks : at.units);
+                const uint32_t place = before + (whole ? at.blocks : at.units);
                 if (place <= in_head && in_head < place + (whole ? mine.blocks : mine.units)) sh.found = q, sh.found_at = place;
                 before += whole ? sum.blocks : sum.units;
                 if (in_head < before) break;
@@ -248,19 +252,19 @@ struct Line {
         }
         c.seq = q;
         c.blocks = blocks_of<ROWS>(p, c.seq);
-        uint64_t rest = in_head - found_at;
+        uint32_t rest = in_head - found_at;
         if (whole || c.blocks == 1) {
-            c.block = whole ? (uint32_t)rest : 0, c.u0 = whole ? 0 : (uint32_t)rest;
+            c.block = whole ? rest : 0, c.u0 = whole ? 0 : rest;
             block_units<ROWS, UNIT>(p, c.seq, c.block, c.first, c.units);
             return true;
         }
         for (uint32_t b0 = 0;; b0 += 32) {  // every warp for itself
             uint32_t first = 0, units = 0;
             if (b0 + lane < c.blocks) block_units<ROWS, UNIT>(p, c.seq, b0 + lane, first, units);
-            uint64_t run = units;
+            uint32_t run = units;
 #pragma unroll
             for (uint32_t o = 1; o < 32; o *= 2) {
-                const uint64_t t = __shfl_up_sync(0xffffffffu, run, o);
+                const uint32_t t = __shfl_up_sync(0xffffffffu, run, o);
                 if (lane >= o) run += t;
             }
             const uint32_t past = __ballot_sync(0xffffffffu, run > rest);
@@ -268,7 +272,7 @@ struct Line {
                 const uint32_t l = past ? __ffs(past) - 1 : 0;
                 c.block = b0 + l;
                 c.first = __shfl_sync(0xffffffffu, first, l), c.units = __shfl_sync(0xffffffffu, units, l);
-                c.u0 = (uint32_t)(rest - (__shfl_sync(0xffffffffu, run, l) - c.units));
+                c.u0 = rest - (__shfl_sync(0xffffffffu, run, l) - c.units);
                 break;
             }
             rest -= __shfl_sync(0xffffffffu, run, 31);
@@ -324,8 +328,8 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi)
 /// Row r of a sequence and key head: its row of q and out, in heads.
 __device__ __forceinline__ void row_at(const Params &p, const Seq &q, uint32_t kv_head, uint32_t r, uint32_t &token, uint32_t &head)
 {
-    token = r / p.group;
-    head = kv_head * p.group + (r - token * p.group);
+    token = p.group.div(r);
+    head = kv_head * p.group.d + (r - token * p.group.d);
     token += q.row0;
 }
 
@@ -361,7 +365,7 @@ __device__ void finish_parts(const Params &p, const L &l, const Pending *pending
         if (came[i] != last - first + 1) continue;
         // Four fours of columns of a row each: 32 bytes of the result, a sector.
         const Seq &q = w.c.seq;
-        const uint32_t rows = min(q.news * p.group - w.c.block * ROWS, ROWS), wide = (d + 15) / 16;
+        const uint32_t rows = min(q.news * p.group.d - w.c.block * ROWS, ROWS), wide = (d + 15) / 16;
         for (uint32_t z = tid; z < ROWS * wide; z += threads) {
             const uint32_t r = z % ROWS, x0 = z / ROWS * 4;
             if (r >= rows) continue;

@@ -113,9 +113,9 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
 
     L line;
     Cursor cur;
-    uint64_t u;
+    uint32_t u;
     if (!line.start(p, blockIdx.x, shared, u, cur)) return;
-    const uint64_t u_end = line.cut(blockIdx.x + 1);
+    const uint32_t u_end = line.cut(blockIdx.x + 1);
     if (u >= u_end) return;
     bool has[2] = {cur.u0 > 0, false};
     if (tid == 0) pending[0] = Pending{cur, u - cur.u0};
@@ -124,9 +124,9 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
     while (true) {
         const uint32_t n_units = line.units_to(cur, u, u_end);
         const Seq &seq = cur.seq;
-        const uint32_t kv_head = cur.kv_head, u0 = cur.u0, rows = seq.news * p.group, row0 = cur.block * ROWS;
+        const uint32_t kv_head = cur.kv_head, u0 = cur.u0, rows = seq.news * p.group.d, row0 = cur.block * ROWS;
         // Keys of this part that the block's rows may see.
-        const uint32_t i0 = row0 / p.group, i1 = (min(row0 + ROWS, rows) - 1) / p.group;
+        const uint32_t i0 = p.group.div(row0), i1 = p.group.div(min(row0 + ROWS, rows) - 1);
         uint32_t lo, hi;
         key_range(p, seq, i0, i1, lo, hi);
         const uint32_t key0 = max((cur.first + u0) * UNIT, lo / kStep * kStep), key1 = min((cur.first + u0 + n_units) * UNIT, hi);
@@ -144,8 +144,8 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
             Where w{p.cache.num_pages, 0};
             const uint32_t l = TMA ? lane : lane & 15u, key = key_of(j) + l * span;
             if (j < mine && l < boxes && key < (TMA ? seq.keys : key1)) {
-                const uint32_t page = (uint32_t)__ldcg(table + page_index(p, key));
-                if (page < p.cache.num_pages) w.page = page, w.slot = page_slot(p, key);
+                const uint32_t page = (uint32_t)__ldcg(table + p.page.div(key));
+                if (page < p.cache.num_pages) w.page = page, w.slot = p.page.mod(key);
             }
             return w;
         };
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
         uint32_t lo_r[2], hi_r[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t i = min(row0 + lane / 4 + 8 * h, rows - 1) / p.group;
+            const uint32_t i = p.group.div(min(row0 + lane / 4 + 8 * h, rows - 1));
             key_range(p, seq, i, i, lo_r[h], hi_r[h]);
         }
         uint32_t lo_all, hi_all;  // what every row of the block sees
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
                 gone = sp.box == 8 ? (b & 1u ? 0xffu : 0u) | (b & 2u ? 0xff00u : 0u) : b ? 0xffffu : 0u;
             } else if (row_hole) {
                 const uint32_t k = key + (lane & 15u);
-                gone = __ballot_sync(0xffffffffu, k < key1 && (uint32_t)__ldcg(table + page_index(p, k)) >= p.cache.num_pages) & 0xffffu;
+                gone = __ballot_sync(0xffffffffu, k < key1 && (uint32_t)__ldcg(table + p.page.div(k)) >= p.cache.num_pages) & 0xffffu;
             }
             float sc[2][4] = {};
             const uint32_t ka = ring + kt * C::TILE;

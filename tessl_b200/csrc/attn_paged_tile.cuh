@@ -28,7 +28,7 @@ namespace tessl {
 namespace attn {
 
 constexpr uint32_t kTileKeys = 128;
-constexpr uint32_t kTileExtra = 6;  // a second part of an item costs as much as six tiles of keys
+constexpr uint32_t kTileExtra = 12;  // a second part of an item costs as much as twelve tiles of keys
 
 template <int DP>
 struct TileCfg {
@@ -239,11 +239,11 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
 
     L line;
     Cursor cur;
-    uint64_t u = 0, u_end = 0;
+    uint32_t u = 0, u_end = 0;
     bool has[2] = {false, false};
     if (line.start(p, blockIdx.x, *reinterpret_cast<typename L::Shared *>(smem_raw + C::Q_BYTES), u, cur)) u_end = line.cut(blockIdx.x + 1);
-    const uint64_t u_start = u;
-    if (tid == 0) pending[1].from = ~0ull;
+    const uint32_t u_start = u;
+    if (tid == 0) pending[1].from = ~0u;
     if (u < u_end) {
         has[0] = cur.u0 > 0;
         if (tid == 0) pending[0] = Pending{cur, u - cur.u0};
@@ -254,9 +254,9 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
     uint32_t n_units, n, steps, k0, row0, rows;
     auto item = [&] {
         n_units = line.units_to(cur, u, u_end);
-        rows = cur.seq.news * p.group, row0 = cur.block * C::ROWS;
+        rows = cur.seq.news * p.group.d, row0 = cur.block * C::ROWS;
         uint32_t lo, hi;
-        key_range(p, cur.seq, row0 / p.group, (min(row0 + C::ROWS, rows) - 1) / p.group, lo, hi);
+        key_range(p, cur.seq, p.group.div(row0), p.group.div(min(row0 + C::ROWS, rows) - 1), lo, hi);
         k0 = (cur.first + cur.u0) * kTileKeys;
         const uint32_t k1 = min(k0 + n_units * kTileKeys, hi);
         n = k1 > k0 ? (k1 - k0 + kTileKeys - 1) / kTileKeys : 0;
@@ -299,8 +299,8 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                 const uint32_t key = k0 + j * kTileKeys + lane * tp.box;
                 page = (int)p.cache.num_pages, slot = 0;
                 if (j < n && lane < boxes && key < cur.seq.keys) {
-                    const uint32_t pg = (uint32_t)__ldcg(table + page_index(p, key));
-                    if (pg < p.cache.num_pages) page = (int)pg, slot = (int)page_slot(p, key);
+                    const uint32_t pg = (uint32_t)__ldcg(table + p.page.div(key));
+                    if (pg < p.cache.num_pages) page = (int)pg, slot = (int)p.page.mod(key);
                 }
             };
             constexpr uint32_t A = C::AHEAD;
@@ -495,12 +495,12 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
             if (mine) {
                 uint32_t lo_r, hi_r;  // rows past the last see what that sees
                 {
-                    const uint32_t i = min(row, rows - 1) / p.group;
+                    const uint32_t i = p.group.div(min(row, rows - 1));
                     key_range(p, cur.seq, i, i, lo_r, hi_r);
                 }
                 const uint32_t lo_all = __shfl_sync(0xffffffffu, lo_r, 31), hi_all = __shfl_sync(0xffffffffu, hi_r, 0);
                 const int32_t *table = p.seqs.table + (size_t)cur.seq.index * p.seqs.max_pages;
-                auto page_of = [&](uint32_t key) { return key < cur.seq.keys ? (uint32_t)__ldcg(table + page_index(p, key)) : 0u; };
+                auto page_of = [&](uint32_t key) { return key < cur.seq.keys ? (uint32_t)__ldcg(table + p.page.div(key)) : 0u; };
                 bool any_hole = false;  // a page of the item is not there: its tiles look at theirs
                 for (uint32_t key = k0 + lane * tp.box; key < k0 + n * kTileKeys; key += 32 * tp.box) any_hole |= page_of(key) >= p.cache.num_pages;
                 any_hole = __any_sync(0xffffffffu, any_hole);
@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(pf::kTmemCols) : "memory");
     }
     if (*abortp || u_start >= u_end) return;
-    has[1] = pending[1].from != ~0ull;
+    has[1] = pending[1].from != ~0u;
     finish_parts<DP, C::ROWS>(p, line, pending, has, C::THREADS, reinterpret_cast<volatile uint32_t *>(smem_raw + C::SMEM - 16));
 }
 
