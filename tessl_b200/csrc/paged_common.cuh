@@ -21,15 +21,24 @@ struct Seqs {
     uint64_t capacity;  // tokens that a row of the table has room for
 };
 
+/// A word that every block reads, through L1 (from L2, some thousand warps wait for one another at the few lines that hold
+/// such words), and after the wait for the launch in front (see dev::ld_after_wait16).
+__device__ __forceinline__ int32_t ld_shared_word(const int32_t *p)
+{
+    int32_t v;
+    asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+
 /// Offsets and lengths come from device memory: whatever they hold, what is made of them stays inside the call's tokens and the
 /// table's row.
 __device__ __forceinline__ uint32_t start_of(const Seqs &q, uint32_t s)
 {
     if (!q.starts) return s;
-    return (uint32_t)min(max(__ldcg(q.starts + s), 0), (int32_t)min(q.total_new, 0x7fffffffu));
+    return (uint32_t)min(max(ld_shared_word(q.starts + s), 0), (int32_t)min(q.total_new, 0x7fffffffu));
 }
 /// Tokens of a sequence by its length; those past q.capacity have no slot.
-__device__ __forceinline__ uint32_t len_of(const Seqs &q, uint32_t s) { return (uint32_t)max(__ldcg(q.lens + s), 0); }
+__device__ __forceinline__ uint32_t len_of(const Seqs &q, uint32_t s) { return (uint32_t)max(ld_shared_word(q.lens + s), 0); }
 
 /// The sequence whose new tokens hold `row`, found by a converged warp, 32 offsets at a time; num_seqs if there is none.
 __device__ __forceinline__ uint32_t seq_of_row(const Seqs &q, uint32_t row)

@@ -2,23 +2,25 @@
 //
 // Pair i of a head turns by position * w_i radians. The angle is kept in turns as a 64-bit fraction: steps[i] =
 // round(2^64 w_i / 2 pi), and position * steps[i] modulo 2^64 is the angle modulo one turn with an error below position * 2^-65 turns,
-// for any 32-bit position. (position * w_i in f32 is off by 0.06 radians at position 10^6.) Sine and cosine of pi times a
-// fraction in [-1, 1) follow in f32.
+// for any 32-bit position. (position * w_i in f32 is off by 0.06 radians at position 10^6.) Its high 32 bits, 2^-32 turns or 1.5e-9
+// radians, are enough for f32: two of them are the quadrant, the rest the sine and cosine of an eighth of a turn at most.
 //
-// One kernel for both operators: a token's heads are spread over groups of lanes, a lane holds two runs of four columns of a head,
-// which are the two halves of four pairs or four whole ones, so a rotation needs no exchange and the norm one butterfly.
-// The angles are computed once per token and shared by its heads. Bound by memory from some thousand tokens on, by the
-// chain offset -> length -> page id -> store (four round trips to L2) below.
+// One kernel for both operators: a warp has a token, or a share of its heads where tokens are few. A lane holds two runs of four columns
+// of a head, which are the two halves of four pairs or four whole pairs, so a rotation needs no exchange, the norm one butterfly, and
+// the lane's cosines and sines serve all heads of the token. The heads' values are on their way while the position is
+// found (offset -> length -> page id, three round trips to L2). Bound by memory from some thousand tokens on, by those
+// round trips below. (With a block per token, whose threads shared the angles through shared memory and a barrier, 8192 x 32 heads of
+// 128 took 46 us.)
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "paged_common.cuh"
 
 namespace tessl {
 namespace {
 
-constexpr uint32_t kThreads = 256;
-constexpr uint32_t kMaxTokens = 8;   // tokens per block, at most: one per warp
+constexpr uint32_t kThreads = 128;
 constexpr uint32_t kMaxPairs = 128;  // of a head of 256
 
 struct HeadsParams {
@@ -34,31 +36,39 @@ struct HeadsParams {
     const float *norm_w[2];  // of q, of k; null: no norm
     float eps, factor;
     uint32_t tokens, dim, rot, interleaved;
-    uint32_t lanes;             // per head, a power of two
-    uint32_t tokens_per_block;  // a power of two
-    uint32_t splits;            // blocks that share the heads of a token
+    uint32_t lanes;   // per head, a power of two
+    uint32_t splits;  // warps that share the heads of a token
 };
 
+/// A run of VEC columns as it lies in memory: 16 bytes, or 8, or one value.
 template <bool IN16, int VEC>
-struct Piece {  // two runs of VEC columns
-    float a[VEC], b[VEC];
-};
-
-template <bool IN16, int VEC>
-__device__ __forceinline__ void load_run(const void *src, size_t at, float (&v)[VEC])
-{
-    if constexpr (VEC == 4 && IN16) {
-        const uint2 w = dev::ld_after_wait8(static_cast<const uint16_t *>(src) + at);
-        v[0] = dev::bf16_lo(w.x), v[1] = dev::bf16_hi(w.x), v[2] = dev::bf16_lo(w.y), v[3] = dev::bf16_hi(w.y);
-    } else if constexpr (VEC == 4) {
-        const uint4 w = dev::ld_after_wait16(static_cast<const float *>(src) + at);
-        v[0] = __uint_as_float(w.x), v[1] = __uint_as_float(w.y), v[2] = __uint_as_float(w.z), v[3] = __uint_as_float(w.w);
-    } else if constexpr (IN16) {
-        v[0] = __uint_as_float((uint32_t)__ldcg(static_cast<const unsigned short *>(src) + at) << 16);
-    } else {
-        v[0] = __ldcg(static_cast<const float *>(src) + at);
+struct Run {
+    uint32_t w[VEC == 1 ? 1 : IN16 ? VEC / 2 : VEC];
+    __device__ __forceinline__ void load(const void *src, size_t at)
+    {
+        if constexpr (VEC == 4 && IN16) {
+            const uint2 v = dev::ld_after_wait8(static_cast<const uint16_t *>(src) + at);
+            w[0] = v.x, w[1] = v.y;
+        } else if constexpr (VEC > 1) {
+            const uint4 v = IN16 ? dev::ld_after_wait16(static_cast<const uint16_t *>(src) + at) : dev::ld_after_wait16(static_cast<const float *>(src) + at);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else if constexpr (IN16) {
+            w[0] = (uint32_t)__ldcg(static_cast<const unsigned short *>(src) + at) << 16;
+        } else {
+            w[0] = __float_as_uint(__ldcg(static_cast<const float *>(src) + at));
+        }
     }
-}
+    __device__ __forceinline__ void get(float (&v)[VEC]) const
+    {
+        if constexpr (VEC > 1 && IN16) {
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) v[2 * i] = dev::bf16_lo(w[i]), v[2 * i + 1] = dev::bf16_hi(w[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = __uint_as_float(w[i]);
+        }
+    }
+};
 
 /// Two f32 -> a bf16 pair, to nearest even.
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi)
@@ -71,10 +81,15 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi)
 template <bool OUT16, int VEC>
 __device__ __forceinline__ void store_run(void *dst, size_t at, const float (&v)[VEC])
 {
-    if constexpr (VEC == 4 && OUT16) {
+    if constexpr (VEC == 8 && OUT16) {
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(dst) + at) =
+            make_uint4(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7]));
+    } else if constexpr (VEC == 4 && OUT16) {
         *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(dst) + at) = make_uint2(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]));
-    } else if constexpr (VEC == 4) {
-        *reinterpret_cast<float4 *>(static_cast<float *>(dst) + at) = make_float4(v[0], v[1], v[2], v[3]);
+    } else if constexpr (VEC > 1) {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4)
+            *reinterpret_cast<float4 *>(static_cast<float *>(dst) + at + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
     } else if constexpr (OUT16) {
         static_cast<uint16_t *>(dst)[at] = (uint16_t)bf16_pair(v[0], 0.0f);
     } else {
@@ -82,192 +97,228 @@ __device__ __forceinline__ void store_run(void *dst, size_t at, const float (&v)
     }
 }
 
-/// VEC = 4: rot a multiple of 8 and everything aligned for whole runs. VEC = 1: anything else, 32 lanes per head.
-/// PAGED: rows find their sequence, positions come from the lengths, k and v go to the cache; else positions are given.
-template <bool IN16, bool OUT16, int VEC, bool PAGED>
+/// factor * (cos, sin) of 2 pi angle / 2^32. Polynomials with the least relative error for |x| <= 1/4 (Remez): sin(pi x) = x P(x^2) to
+/// 3e-9, cos(pi x) = Q(x^2) to 6e-11; with the rounding in f32 both are within 2 * 2^-24.
+__device__ __forceinline__ float2 turn_of(uint32_t angle, float factor)
+{
+    const uint32_t quadrant = (angle + 0x20000000u) >> 30;
+    const float x = (float)(int32_t)(angle - (quadrant << 30)) * 0x1p-31f, t = x * x;
+    float s = fmaf(fmaf(fmaf(-0.5890122056f, t, 2.5497610569f), t, -5.1677079201f), t, 3.1415927410f) * x;
+    float c = fmaf(fmaf(fmaf(fmaf(0.2312609255f, t, -1.3350359201f), t, 4.0587067604f), t, -4.9348020554f), t, 1.0f);
+    const float sf = quadrant & 2u ? -factor : factor, cf = (quadrant + 1) & 2u ? -factor : factor;
+    return quadrant & 1u ? make_float2(cf * s, sf * c) : make_float2(cf * c, sf * s);
+}
+
+/// Through L1: all warps read the same few lines (from L2, 8192 tokens x 32 heads of 128 took 31 us instead of 27).
+__device__ __forceinline__ uint64_t step_of(const uint64_t *p)
+{
+    uint64_t v;
+    asm volatile("ld.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+    return v;
+}
+
+/// VEC = 8 (bf16 in) or 4: rot and the rest of a head multiples of 2 VEC and everything aligned for whole runs. VEC = 1: anything else,
+/// 32 lanes per head. PAGED: rows find their sequence, positions come from the lengths, k and v go to the cache; else positions are given.
+/// NORM: heads of q and k are normed first.
+template <bool IN16, bool OUT16, int VEC, bool PAGED, bool NORM>
 __global__ void __launch_bounds__(kThreads) rope_heads_kernel(const HeadsParams p)
 {
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    constexpr int UPL = VEC == 4 ? 1 : 4;  // pieces per lane: a head of 256 has 32 of 8 columns, 128 of 2
-    __shared__ float2 turn[kMaxTokens][kMaxPairs];  // factor * (cos, sin)
-    __shared__ int64_t place[kMaxTokens];           // of the token's row in the cache; -1: none
-    __shared__ uint32_t live[kMaxTokens];           // the row belongs to a sequence
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t tpb = p.tokens_per_block, t0 = blockIdx.x * tpb;
-    const uint32_t lanes = p.lanes, groups = kThreads / lanes, group = tid / lanes, sub = tid & (lanes - 1);
-    const uint32_t nq = p.heads[0], nkv = p.heads[1], nh = nq + 2 * nkv;  // heads of a token
+    constexpr int UPL = VEC > 1 ? 1 : 4;     // pieces (two runs) per lane: a head of 256 has 128 of 2 columns
+    constexpr int BATCH = VEC == 1 ? 1 : 2;  // rounds whose loads are issued together, a batch ahead
+    const uint32_t lane = threadIdx.x & 31;
+    const uint64_t w = (uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    const uint32_t token = (uint32_t)(w / p.splits), split = (uint32_t)(w - (uint64_t)token * p.splits);
+    if (token >= p.tokens) return;
+    const uint32_t lanes = p.lanes, at_once = 32 / lanes, sub = lane & (lanes - 1), group = lane / lanes;  // heads at once
+    const uint32_t nq = p.heads[0], nkv = p.heads[1];
     const uint32_t units = p.dim / (2 * VEC), rot_units = p.rot / (2 * VEC), half = p.rot / 2;
-    // Work item w of the block's share: head w % nh of token w / nh.
-    const uint32_t items = tpb * nh, first = blockIdx.y * groups + group, step = groups * p.splits;
+    // A round is at_once heads of q, k or v.
+    const uint32_t rounds_q = (nq + at_once - 1) / at_once, rounds_kv = (nkv + at_once - 1) / at_once, rounds = rounds_q + 2 * rounds_kv;
 
-    auto columns = [&](uint32_t u, uint32_t &a, uint32_t &b) {  // the two runs of piece u
-        if (u < rot_units) {
-            a = p.interleaved ? 2 * VEC * u : VEC * u;
-            b = p.interleaved ? a + VEC : half + a;
-        } else {
-            a = p.rot + 2 * VEC * (u - rot_units), b = a + VEC;
-        }
-    };
-    auto which = [&](uint32_t head, uint32_t &h) {  // 0 q, 1 k, 2 v; h: the head among them
-        if (head < nq) return h = head, 0u;
-        h = head - nq;
-        if (h < nkv) return 1u;
-        h -= nkv;
-        return 2u;
-    };
-    Piece<IN16, VEC> cur[UPL];
-    auto fetch = [&](uint32_t w, Piece<IN16, VEC> (&v)[UPL]) {
-        const uint32_t token = t0 + w / nh;
-        uint32_t h;
-        const uint32_t kind = which(w % nh, h);
-        if (token >= p.tokens) return;
-        const void *src = kind == 0 ? p.src[0] : kind == 1 ? p.src[1] : p.src[2];
-        const size_t row = (size_t)token * (kind == 0 ? p.src_stride[0] : kind == 1 ? p.src_stride[1] : p.src_stride[2]) + (size_t)h * p.dim;
+    uint32_t ca[UPL], cb[UPL];  // the first columns of this lane's runs
 #pragma unroll
-        for (int i = 0; i < UPL; ++i) {
-            const uint32_t u = sub + i * 32;
-            if (u >= units) continue;
-            uint32_t a, b;
-            columns(u, a, b);
-            load_run<IN16, VEC>(src, row + a, v[i].a), load_run<IN16, VEC>(src, row + b, v[i].b);
-        }
-    };
-    if (first < items) fetch(first, cur);  // in flight while the positions are found
-
-    {   // warp w looks after token w % tpb, with the other warps of that token a share of its angles
-        const uint32_t tl = warp & (tpb - 1), row = t0 + tl, share = kThreads / 32 / tpb;
-        int32_t pos = 0;
-        bool alive = row < p.tokens;
-        if (PAGED && alive) {
-            const uint32_t s = paged::seq_of_row(p.seqs, row);
-            alive = s < p.seqs.num_seqs;
-            if (alive) {
-                const uint32_t len = paged::len_of(p.seqs, s), end = p.seqs.starts ? paged::start_of(p.seqs, s + 1) : s + 1;
-                pos = (int32_t)(len - (end - row));  // below 0: in front of the sequence
-                if (lane == 0 && warp < tpb) {
-                    int64_t at = -1;
-                    if (pos >= 0 && (uint64_t)pos < p.seqs.capacity) {
-                        const uint32_t page = (uint32_t)__ldcg(p.seqs.table + (size_t)s * p.seqs.max_pages + (uint32_t)pos / p.cache.page_size);
-                        if (page < p.cache.num_pages)
-                            at = (int64_t)(page * p.cache.page_stride + (uint64_t)((uint32_t)pos % p.cache.page_size) * p.cache.token_stride);
-                    }
-                    place[tl] = at;
-                }
-            }
-        } else if (alive) {
-            pos = __ldcg(p.positions + row);
-        }
-        if (lane == 0 && warp < tpb) live[tl] = alive;
-        for (uint32_t i = (warp / tpb) * 32 + lane; i < half && alive; i += share * 32) {
-            const uint64_t t = (uint64_t)(int64_t)pos * __ldcg(reinterpret_cast<const unsigned long long *>(p.steps) + i);
-            float s, c;
-            sincospif(__ll2float_rn((long long)t) * 0x1p-63f, &s, &c);
-            turn[tl][i] = make_float2(p.factor * c, p.factor * s);
+    for (int i = 0; i < UPL; ++i) {
+        const uint32_t u = sub + i * 32;
+        // Runs lie side by side over the lanes: of the two halves, whatever the pairs are. (Whole pairs in neighbouring runs read and wrote
+        // half sectors.) Runs of one column: a pair.
+        if (u < rot_units) {
+            const bool pair = VEC == 1 && p.interleaved;
+            ca[i] = pair ? 2 * u : VEC * u, cb[i] = pair ? 2 * u + 1 : half + VEC * u;
+        } else {
+            ca[i] = p.rot + VEC * (u - rot_units), cb[i] = ca[i] + (p.dim - p.rot) / 2;
         }
     }
-    __syncthreads();
-
-    for (uint32_t w = first; w < items; w += step) {
-        Piece<IN16, VEC> next[UPL];
-        if (w + step < items) fetch(w + step, next);
-        const uint32_t tl = w / nh, token = t0 + tl;
-        uint32_t h;
-        const uint32_t kind = which(w % nh, h);
-        const bool alive = token < p.tokens && live[tl];
-        if (PAGED && kind < 2 && p.norm_w[0]) {
-            float ss = 0.0f;
+    const size_t row_q = (size_t)token * p.src_stride[0], row_k = (size_t)token * p.src_stride[1], row_v = (size_t)token * p.src_stride[2];
+    // Of a round: 0 q, 1 k, 2 v, and this lane's head among them.
+    auto which = [&](uint32_t round, uint32_t &head) {
+        const uint32_t kind = round < rounds_q ? 0u : round < rounds_q + rounds_kv ? 1u : 2u;
+        head = (round - (kind == 0 ? 0 : kind == 1 ? rounds_q : rounds_q + rounds_kv)) * at_once + group;
+        return kind;
+    };
+    using R = Run<IN16, VEC>;
+    R ra[2][BATCH][UPL], rb[2][BATCH][UPL];
+    auto fetch = [&](uint32_t round0, R (&a)[BATCH][UPL], R (&b)[BATCH][UPL]) {
+#pragma unroll
+        for (int y = 0; y < BATCH; ++y) {
+            const uint32_t round = round0 + y * p.splits;
+            if (round >= rounds) continue;
+            uint32_t head;
+            const uint32_t kind = which(round, head);
+            if (head >= (kind == 0 ? nq : nkv)) continue;
+            const void *src = kind == 0 ? p.src[0] : kind == 1 ? p.src[1] : p.src[2];
+            const size_t row = (kind == 0 ? row_q : kind == 1 ? row_k : row_v) + head * p.dim;
 #pragma unroll
             for (int i = 0; i < UPL; ++i)
+                if (sub + i * 32 < units) a[y][i].load(src, row + ca[i]), b[y][i].load(src, row + cb[i]);
+        }
+    };
+    fetch(split, ra[0], rb[0]);  // in flight while the position is found
+
+    int32_t pos = 0;
+    int64_t place = -1;  // of the token's row in the cache; -1: none
+    if constexpr (PAGED) {
+        const uint32_t s = paged::seq_of_row(p.seqs, token);
+        if (s >= p.seqs.num_seqs) return;  // behind the last sequence
+        const uint32_t len = paged::len_of(p.seqs, s), end = p.seqs.starts ? paged::start_of(p.seqs, s + 1) : s + 1;
+        pos = (int32_t)(len - (end - token));  // below 0: in front of the sequence
+        if (pos >= 0 && (uint64_t)pos < p.seqs.capacity) {
+            const uint32_t page = (uint32_t)__ldcg(p.seqs.table + (size_t)s * p.seqs.max_pages + (uint32_t)pos / p.cache.page_size);
+            if (page < p.cache.num_pages)
+                place = (int64_t)(page * p.cache.page_stride + (uint64_t)((uint32_t)pos % p.cache.page_size) * p.cache.token_stride);
+        }
+    } else {
+        pos = __ldcg(p.positions + token);
+    }
+    float2 turn[UPL][VEC];  // factor * (cos, sin) of this lane's pairs
 #pragma unroll
-                for (int e = 0; e < VEC; ++e)
-                    if (sub + i * 32 < units) ss = fmaf(cur[i].a[e], cur[i].a[e], ss), ss = fmaf(cur[i].b[e], cur[i].b[e], ss);
-            const uint32_t mask = lanes == 32 ? 0xffffffffu : ((1u << lanes) - 1u) << (lane & ~(lanes - 1));
-            for (uint32_t o = lanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-            const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, (float)p.dim) + p.eps));
-            const float *nw = kind == 0 ? p.norm_w[0] : p.norm_w[1];
+    for (int i = 0; i < UPL; ++i) {
+        if (sub + i * 32 >= rot_units) continue;
 #pragma unroll
-            for (int i = 0; i < UPL; ++i) {
-                const uint32_t u = sub + i * 32;
-                if (u >= units) continue;
-                uint32_t a, b;
-                columns(u, a, b);
+        for (int e = 0; e < VEC; ++e) {
+            uint32_t pair = (sub + i * 32) * VEC + e;
+            if (VEC > 1 && p.interleaved) pair = (e < VEC / 2 ? ca[i] : cb[i]) / 2 + e % (VEC > 1 ? VEC / 2 : 1);
+            const uint64_t t = (uint64_t)(int64_t)pos * step_of(p.steps + pair);
+            turn[i][e] = turn_of((uint32_t)(t >> 32), p.factor);
+        }
+    }
+    float wq[UPL][2 * VEC], wk[UPL][2 * VEC];  // 1 + the norms' weights of this lane's columns
+    if constexpr (NORM) {
+        auto load = [](const float *at) {
+            float v;
+            asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(at) : "memory");  // not before the wait above
+            return 1.0f + v;
+        };
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    cur[i].a[e] = __fmul_rn(__fmul_rn(cur[i].a[e], inv), 1.0f + __ldcg(nw + a + e));
-                    cur[i].b[e] = __fmul_rn(__fmul_rn(cur[i].b[e], inv), 1.0f + __ldcg(nw + b + e));
-                }
+        for (int i = 0; i < UPL; ++i) {
+            if (sub + i * 32 >= units) continue;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                wq[i][e] = load(p.norm_w[0] + ca[i] + e), wq[i][VEC + e] = load(p.norm_w[0] + cb[i] + e);
+                wk[i][e] = load(p.norm_w[1] + ca[i] + e), wk[i][VEC + e] = load(p.norm_w[1] + cb[i] + e);
             }
         }
-        const int64_t at = PAGED ? place[tl] : 0;
-        if (alive && (kind == 0 || at >= 0)) {
+    }
+
+    auto process = [&](uint32_t round0, const R (&ia)[BATCH][UPL], const R (&ib)[BATCH][UPL]) {
+#pragma unroll
+        for (int y = 0; y < BATCH; ++y) {
+            const uint32_t round = round0 + y * p.splits;
+            if (round >= rounds) continue;
+            uint32_t head;
+            const uint32_t kind = which(round, head);
+            const bool there = head < (kind == 0 ? nq : nkv) && (kind == 0 || place >= 0);
+            float a[UPL][VEC], b[UPL][VEC];
+#pragma unroll
+            for (int i = 0; i < UPL; ++i) ia[y][i].get(a[i]), ib[y][i].get(b[i]);
+            if (NORM && kind < 2) {  // the whole warp: heads that are not there are summed for nothing
+                float ss = 0.0f;
+#pragma unroll
+                for (int i = 0; i < UPL; ++i)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        if (sub + i * 32 < units) ss = fmaf(a[i][e], a[i][e], ss), ss = fmaf(b[i][e], b[i][e], ss);
+                for (uint32_t o = lanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, (float)p.dim) + p.eps));
+#pragma unroll
+                for (int i = 0; i < UPL; ++i)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        a[i][e] = __fmul_rn(__fmul_rn(a[i][e], inv), kind == 0 ? wq[i][e] : wk[i][e]);
+                        b[i][e] = __fmul_rn(__fmul_rn(b[i][e], inv), kind == 0 ? wq[i][VEC + e] : wk[i][VEC + e]);
+                    }
+            }
+            if (!there) continue;
 #pragma unroll
             for (int i = 0; i < UPL; ++i) {
                 const uint32_t u = sub + i * 32;
                 if (u >= units) continue;
-                uint32_t a, b;
-                columns(u, a, b);
-                Piece<IN16, VEC> &c = cur[i];
                 if (kind < 2 && u < rot_units) {
                     if (VEC == 1 || !p.interleaved) {
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) {
-                            const float2 cs = turn[tl][u * VEC + e];
-                            const float x = c.a[e], y = c.b[e];
-                            c.a[e] = x * cs.x - y * cs.y, c.b[e] = x * cs.y + y * cs.x;
+                            const float2 cs = turn[i][e];
+                            const float x = a[i][e], z = b[i][e];
+                            a[i][e] = x * cs.x - z * cs.y, b[i][e] = x * cs.y + z * cs.x;
                         }
                     } else {
                         constexpr int H = VEC / 2;
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) {
-                            const float2 cs = turn[tl][u * VEC + e];
-                            float &x = e < H ? c.a[(2 * e) % VEC] : c.b[(2 * e) % VEC], &y = e < H ? c.a[(2 * e + 1) % VEC] : c.b[(2 * e + 1) % VEC];
-                            const float x0 = x, y0 = y;
-                            x = x0 * cs.x - y0 * cs.y, y = x0 * cs.y + y0 * cs.x;
+                            const float2 cs = turn[i][e];
+                            float &x = e < H ? a[i][(2 * e) % VEC] : b[i][(2 * e) % VEC], &z = e < H ? a[i][(2 * e + 1) % VEC] : b[i][(2 * e + 1) % VEC];
+                            const float x0 = x, z0 = z;
+                            x = x0 * cs.x - z0 * cs.y, z = x0 * cs.y + z0 * cs.x;
                         }
                     }
                 }
                 if (!PAGED || kind == 0) {
-                    const size_t row = (size_t)token * p.out_stride + (size_t)h * p.dim;
-                    store_run<OUT16, VEC>(p.out, row + a, c.a), store_run<OUT16, VEC>(p.out, row + b, c.b);
+                    const size_t row = (size_t)token * p.out_stride + head * p.dim;
+                    store_run<OUT16, VEC>(p.out, row + ca[i], a[i]), store_run<OUT16, VEC>(p.out, row + cb[i], b[i]);
                 } else {
-                    const size_t row = (size_t)at + (size_t)h * p.cache.head_stride;
+                    const size_t row = (size_t)place + head * p.cache.head_stride;
                     uint16_t *dst = kind == 1 ? p.cache.k : p.cache.v;
-                    store_run<true, VEC>(dst, row + a, c.a), store_run<true, VEC>(dst, row + b, c.b);
+                    store_run<true, VEC>(dst, row + ca[i], a[i]), store_run<true, VEC>(dst, row + cb[i], b[i]);
                 }
             }
         }
-#pragma unroll
-        for (int i = 0; i < UPL; ++i) cur[i] = next[i];
+    };
+    for (uint32_t round = split; round < rounds; round += 2 * BATCH * p.splits) {
+        fetch(round + BATCH * p.splits, ra[1], rb[1]);
+        process(round, ra[0], rb[0]);
+        fetch(round + 2 * BATCH * p.splits, ra[0], rb[0]);
+        process(round + BATCH * p.splits, ra[1], rb[1]);
     }
 }
 
+/// `run`: the columns of a run, 8, 4 or 1.
 template <bool PAGED>
-Result launch_heads(TesslRuntime *rt, const char *what, HeadsParams p, bool in16, bool out16, bool wide)
+Result launch_heads(TesslRuntime *rt, const char *what, HeadsParams p, bool in16, bool out16, uint32_t run)
 {
-    const uint32_t nh = p.heads[0] + 2 * p.heads[1];
     p.lanes = 32;
-    if (wide)
-        while (p.lanes > 1 && p.lanes / 2 * 8 >= p.dim) p.lanes /= 2;
-    const uint32_t groups = kThreads / p.lanes;
-    // Tokens of few heads share a block; the heads of few tokens are spread over several, until there is a block for each SM.
-    p.tokens_per_block = 1;
-    while (p.tokens_per_block < kMaxTokens && p.tokens_per_block * 2 * nh <= groups &&
-           p.tokens / (p.tokens_per_block * 2) >= (uint32_t)rt->sm_count)
-        p.tokens_per_block *= 2;
-    const uint32_t blocks = (p.tokens - 1) / p.tokens_per_block + 1, rounds = (p.tokens_per_block * nh - 1) / groups + 1;
-    p.splits = min(min(rounds, 65535u), max(1u, 2 * (uint32_t)rt->sm_count / blocks));
-    auto go = [&](auto kernel) { return launch_pdl(rt, what, kernel, dim3(blocks, p.splits), dim3(kThreads), 0, p); };
-    if (PAGED) {
-        if (wide) return in16 ? go(rope_heads_kernel<true, true, 4, PAGED>) : go(rope_heads_kernel<false, true, 4, PAGED>);
-        return in16 ? go(rope_heads_kernel<true, true, 1, PAGED>) : go(rope_heads_kernel<false, true, 1, PAGED>);
+    if (run > 1)
+        while (p.lanes > 1 && p.lanes / 2 * 2 * run >= p.dim) p.lanes /= 2;
+    // The heads of few tokens are spread over several warps, until there are 16 for each SM.
+    const uint32_t at_once = 32 / p.lanes, rounds = (p.heads[0] + at_once - 1) / at_once + 2 * ((p.heads[1] + at_once - 1) / at_once);
+    p.splits = std::min(rounds, std::max(1u, 16 * (uint32_t)rt->sm_count / p.tokens));
+    const uint64_t blocks = ((uint64_t)p.tokens * p.splits - 1) / (kThreads / 32) + 1;  // below 2^31: p.tokens is
+    auto go = [&](auto kernel) { return launch_pdl(rt, what, kernel, dim3((unsigned)blocks), dim3(kThreads), 0, p); };
+    auto typed = [&](auto in, auto out, auto norm) {
+        constexpr bool IN = decltype(in)::value, OUT = decltype(out)::value, NORM = decltype(norm)::value;
+        if constexpr (IN)
+            if (run == 8) return go(rope_heads_kernel<IN, OUT, 8, PAGED, NORM>);
+        return run > 1 ? go(rope_heads_kernel<IN, OUT, 4, PAGED, NORM>) : go(rope_heads_kernel<IN, OUT, 1, PAGED, NORM>);
+    };
+    const std::true_type yes{};
+    const std::false_type no{};
+    if constexpr (PAGED) {
+        if (p.norm_w[0]) return in16 ? typed(yes, yes, yes) : typed(no, yes, yes);
+        return in16 ? typed(yes, yes, no) : typed(no, yes, no);
+    } else {
+        if (in16) return out16 ? typed(yes, yes, no) : typed(yes, no, no);
+        return out16 ? typed(no, yes, no) : typed(no, no, no);
     }
-    if (wide) {
-        if (in16) return out16 ? go(rope_heads_kernel<true, true, 4, PAGED>) : go(rope_heads_kernel<true, false, 4, PAGED>);
-        return out16 ? go(rope_heads_kernel<false, true, 4, PAGED>) : go(rope_heads_kernel<false, false, 4, PAGED>);
-    }
-    if (in16) return out16 ? go(rope_heads_kernel<true, true, 1, PAGED>) : go(rope_heads_kernel<true, false, 1, PAGED>);
-    return out16 ? go(rope_heads_kernel<false, true, 1, PAGED>) : go(rope_heads_kernel<false, false, 1, PAGED>);
 }
 
 Result rope_validate(const TesslRope &r, uint32_t head_dim, const char *what)
@@ -279,9 +330,20 @@ Result rope_validate(const TesslRope &r, uint32_t head_dim, const char *what)
     return ok();
 }
 
-bool aligned(const void *p, uint32_t stride, bool is16)
+/// Columns of the longest run that memory of 16-bit or 32-bit values allows: 8, 4 or 1.
+uint32_t run_of(const void *p, uint32_t stride, bool is16)
 {
-    return ((uintptr_t)p & (is16 ? 7u : 15u)) == 0 && stride % 4 == 0;
+    const uint32_t size = is16 ? 2 : 4;
+    for (uint32_t run : {8u, 4u})
+        if (((uintptr_t)p & (std::min(run * size, 16u) - 1)) == 0 && stride % (std::min(run * size, 16u) / size) == 0) return run;
+    return 1;
+}
+
+/// The same of a head: whole runs, two by two, in its rotated part and behind it; 8 columns of f32 are two loads, no better than 4.
+uint32_t run_of(uint32_t dim, uint32_t rot, bool in16)
+{
+    if (in16 && dim % 16 == 0 && rot % 16 == 0) return 8;
+    return dim % 8 == 0 && rot % 8 == 0 ? 4 : 1;
 }
 
 }  // namespace
@@ -357,8 +419,8 @@ Result rope(TesslRuntime *rt, const TesslBuf &x, const TesslBuf &positions, cons
     p.out = out.ptr, p.out_stride = out_stride;
     p.positions = static_cast<const int32_t *>(positions.ptr), p.steps = static_cast<const uint64_t *>(rope.steps.ptr);
     p.factor = rope.factor, p.tokens = tokens, p.dim = head_dim, p.rot = rope.rot_dim, p.interleaved = rope.interleaved != 0;
-    const bool wide = head_dim % 8 == 0 && rope.rot_dim % 8 == 0 && aligned(x.ptr, x_stride, x_as_bf16) && aligned(out.ptr, out_stride, out_as_bf16);
-    return launch_heads<false>(rt, "rope launch", p, x_as_bf16, out_as_bf16, wide);
+    const uint32_t run = std::min({run_of(head_dim, rope.rot_dim, x_as_bf16), run_of(x.ptr, x_stride, x_as_bf16), run_of(out.ptr, out_stride, out_as_bf16)});
+    return launch_heads<false>(rt, "rope launch", p, x_as_bf16, out_as_bf16, run);
 }
 
 Result kv_append_paged(TesslRuntime *rt, const TesslBuf &q, const TesslBuf &k, const TesslBuf &v, const TesslBuf &q_out,
@@ -404,9 +466,9 @@ Result kv_append_paged(TesslRuntime *rt, const TesslBuf &q, const TesslBuf &k, c
         p.norm_w[0] = n_heads ? static_cast<const float *>(norm->q_weight.ptr) : p.norm_w[1];
         p.eps = norm->eps;
     }
-    bool wide = p.rot % 8 == 0 && aligned(k.ptr, k_stride, in_as_bf16) && aligned(v.ptr, v_stride, in_as_bf16);
-    if (n_heads) wide = wide && aligned(q.ptr, q_stride, in_as_bf16) && aligned(q_out.ptr, p.out_stride, true);
-    return launch_heads<true>(rt, "kv_append_paged launch", p, in_as_bf16, true, wide);
+    uint32_t run = std::min({run_of(dim, p.rot, in_as_bf16), run_of(k.ptr, k_stride, in_as_bf16), run_of(v.ptr, v_stride, in_as_bf16)});
+    if (n_heads) run = std::min({run, run_of(q.ptr, q_stride, in_as_bf16), run_of(q_out.ptr, p.out_stride, true)});
+    return launch_heads<true>(rt, "kv_append_paged launch", p, in_as_bf16, true, run);
 }
 
 }  // namespace nn
