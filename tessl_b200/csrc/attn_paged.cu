@@ -37,11 +37,18 @@ bool wants_tiles(const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t
     return seqs.q_starts.ptr && cache.num_pages > 0 && cache.page_size % 8 == 0 && elems(total_new, group) > 32ull * seqs.num_seqs;
 }
 
+/// Blocks of the split kernel on an SM.
+uint32_t split_blocks(const TesslRuntime *rt, const TesslPagedKv &cache, const TesslPagedSeqs &seqs)
+{
+    return elems(seqs.num_seqs, cache.n_kv_heads) > (uint64_t)rt->sm_count ? 2 : 1;
+}
+
 uint64_t workspace_of(const TesslRuntime *rt, const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t group)
 {
     return with_dim(cache.head_dim, [&](auto dp) -> uint64_t {
         constexpr int DP = decltype(dp)::value;
-        const uint64_t few = attn::Part<attn::kSplitRows, DP>::bytes(rt->sm_count), many = attn::Part<attn::TileCfg<DP>::ROWS, DP>::bytes(rt->sm_count);
+        const uint64_t few = attn::Part<attn::kSplitRows, DP>::bytes((uint64_t)rt->sm_count * split_blocks(rt, cache, seqs));
+        const uint64_t many = attn::Part<attn::TileCfg<DP>::ROWS, DP>::bytes(rt->sm_count);
         return wants_tiles(cache, seqs, total_new, group) ? std::max(few, many) : few;
     });
 }
@@ -58,21 +65,21 @@ Result cache_maps(TesslRuntime *rt, const char *what, const paged::Cache &c, uin
     return make_map(enc, what, v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c.v, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int DP>
+template <int DP, int BLOCKS>
 Result launch_split(TesslRuntime *rt, const Params &p)
 {
-    using C = attn::SplitCfg<DP>;
+    using C = attn::SplitCfg<DP, BLOCKS>;
     const char *what = "attn_paged launch";
     attn::SplitParams sp{p, box_of(p.cache.page_size, attn::kStep)};
-    sp.p.parts = (uint32_t)rt->sm_count;
+    sp.p.parts = (uint32_t)rt->sm_count * BLOCKS;
     CUtensorMap map_k{}, map_v{};
     auto go = [&](auto kernel) -> Result {
         TESSL_TRY(smem_opt_in(rt, (const void *)kernel, C::SMEM, what, true));
         return launch_pdl(rt, what, kernel, dim3(sp.p.parts), dim3(C::THREADS), C::SMEM, map_k, map_v, sp);
     };
-    if (p.cache.num_pages == 0 || sp.box < 8) return go(attn::attn_paged_split_kernel<DP, false>);
+    if (p.cache.num_pages == 0 || sp.box < 8) return go(attn::attn_paged_split_kernel<DP, false, BLOCKS>);
     TESSL_TRY(cache_maps(rt, what, p.cache, sp.box, &map_k, &map_v));
-    return go(attn::attn_paged_split_kernel<DP, true>);
+    return go(attn::attn_paged_split_kernel<DP, true, BLOCKS>);
 }
 
 template <int DP>
@@ -160,9 +167,10 @@ Result attn_paged(TesslRuntime *rt, const TesslBuf &q, const TesslPagedKv &cache
     p.mark = next_mark(rt);
     // A scale of zero makes zeros of scores that a mask has set to -inf: the tile kernel masks before it scales.
     const bool tiles = wants_tiles(cache, seqs, total_new, p.group.d) && p.scale_log2 != 0.0f;
+    const bool two = split_blocks(rt, cache, seqs) == 2;
     return with_dim(cache.head_dim, [&](auto dp) {
         constexpr int DP = decltype(dp)::value;
-        if (!tiles) return launch_split<DP>(rt, p);
+        if (!tiles) return two ? launch_split<DP, 2>(rt, p) : launch_split<DP, 1>(rt, p);
         const bool negate = p.scale_log2 < 0.0f;
         p.scale_log2 = std::fabs(p.scale_log2);
         return launch_tiles<DP>(rt, p, negate);

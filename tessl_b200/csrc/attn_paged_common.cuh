@@ -123,16 +123,21 @@ struct Line {
         uint32_t many[THREADS], n_many, found_at;
         Seq found;
     };
-    uint32_t per_head, each;
-    uint32_t parts, longer;  // the first `longer` parts have each + 1
-    bool whole;              // items are not cut: the line counts items
+    uint32_t per_head, parts;
+    uint32_t span, cuts;    // every `span` places are cut for themselves, into this many parts:
+    uint32_t each, longer;  // the first `longer` of them have each + 1 places, the others `each`
+    bool whole;             // items are not cut: the line counts items
 
-    __device__ __forceinline__ uint32_t cut(uint32_t c) const { return each * c + min(c, longer); }
+    __device__ __forceinline__ uint32_t cut(uint32_t c) const
+    {
+        const uint32_t i = cuts == parts ? (c >= parts) : c / cuts, k = c - i * cuts;
+        return i * span + each * k + min(k, longer);
+    }
     /// The part that holds place u.
     __device__ __forceinline__ uint32_t part_of(uint32_t u) const
     {
-        const uint32_t edge = (each + 1) * longer;
-        return u < edge ? u / (each + 1) : longer + (u - edge) / each;
+        const uint32_t i = cuts == parts ? 0 : u / span, v = u - i * span, edge = (each + 1) * longer;
+        return i * cuts + (v < edge ? v / (each + 1) : longer + (v - edge) / each);
     }
     /// Units of the item at the cursor that lie between places u and u_end, and how far they reach.
     __device__ __forceinline__ uint32_t units_to(const Cursor &c, uint32_t u, uint32_t u_end) const
@@ -232,9 +237,15 @@ struct Line {
         whole = (items + p.parts - 1) / p.parts * (uint64_t)all.most <= units / p.parts + EXTRA;
         const uint32_t total = whole ? items : units;
         per_head = whole ? all.blocks : all.units;
-        parts = min(p.parts, total);
+        span = total, cuts = min(p.parts, total);
+        // A few items of the same length: no block has parts of two.
+        if (!whole && all.most * all.blocks == all.units && items <= p.parts) {
+            const uint32_t k = min(p.parts / items, all.most);
+            if ((all.most + k - 1) / k <= units / p.parts + EXTRA / 2) span = all.most, cuts = k;
+        }
+        parts = span == total ? cuts : items * cuts;
         if (part >= parts) return false;
-        each = total / parts, longer = total - each * parts;
+        each = span / cuts, longer = span - each * cuts;
         from = cut(part);
         c.kv_head = from / per_head;
         const uint32_t in_head = from - c.kv_head * per_head;
@@ -333,28 +344,40 @@ __device__ __forceinline__ void row_at(const Params &p, const Seq &q, uint32_t k
     token += q.row0;
 }
 
+/// Before a barrier in front of finish_parts, by one thread, for each item (where it begins on the line) of which the block has a part: a counter that does not hold a number of
+/// this call's own and a count holds what another call or nobody has put there, and is given the number and a count of 0 by the first block
+/// to see that. Whoever has added up puts the count back to 0, for a replay of this call has the same number.
+template <uint32_t DP, uint32_t ROWS, typename L>
+__device__ __forceinline__ void expect_parts(const Params &p, const L &l, uint32_t from)
+{
+    unsigned long long *const at = Part<ROWS, DP>::counter(p, l.part_of(from));
+    const unsigned long long seen = __ldcg(at);
+    if (seen >> 16 != p.mark) atomicCAS(at, seen, p.mark << 16);
+}
+
 /// The end of a block: its parts, one of the item that it began in the middle of (pending[0]) and one of the item whose start it has
 /// (pending[1]), are counted in and, where it is the last of an item's blocks to come, added up. All threads call this behind a
-/// barrier that follows the last store to the workspace; `came`: two words of shared memory.
+/// barrier that follows the last store to the workspace; `came`: two words of shared memory, `shared`: `room`
+/// words that nobody uses any longer, 16 for each thread and many times the two of every part's row.
 ///
-/// The counters need no preparation. One holds a number of this call's own and a count; what another call or nobody has put there
-/// has another number and stands for a count of 0. Whoever has added up puts a 0 there, for a replay of this call has the same number.
+/// The counters need no preparation: each of an item's blocks has called expect_parts before. (Counting in by compare and swap alone,
+/// which needs no call before, took the twenty blocks of an item up to 7 us.)
 template <uint32_t DP, uint32_t ROWS, typename L>
 __device__ void finish_parts(const Params &p, const L &l, const Pending *pending, const bool (&has)[2], uint32_t threads,
-                             volatile uint32_t *came)
+                             volatile uint32_t *came, float *shared, uint32_t room)
 {
     using P = Part<ROWS, DP>;
     if (!has[0] && !has[1]) return;
     const uint32_t tid = threadIdx.x, d = p.cache.head_dim;
-    if (tid < 2 && has[tid]) {
+    if (tid == 0) {
         __threadfence();  // the block's parts, behind the barrier that all have passed
-        unsigned long long *const at = P::counter(p, l.part_of(pending[tid].from));
-        unsigned long long seen = 0, old;
-        do {
-            old = seen;
-            seen = atomicCAS(at, old, (old >> 16 == p.mark ? old : p.mark << 16) + 1);
-        } while (seen != old);
-        came[tid] = (uint32_t)(old >> 16 == p.mark ? old & 0xffffu : 0) + 1;
+        unsigned long long old[2];
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i)
+            if (has[i]) old[i] = atomicAdd(P::counter(p, l.part_of(pending[i].from)), 1ull);
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i)
+            if (has[i]) came[i] = (uint32_t)(old[i] & 0xffffu) + 1;
         __threadfence();
     }
     __syncthreads();
@@ -363,44 +386,88 @@ __device__ void finish_parts(const Params &p, const L &l, const Pending *pending
         const Pending &w = pending[i];
         const uint32_t first = l.part_of(w.from), last = l.part_of(w.from + w.c.units - 1);
         if (came[i] != last - first + 1) continue;
-        // Four fours of columns of a row each: 32 bytes of the result, a sector.
         const Seq &q = w.c.seq;
-        const uint32_t rows = min(q.news * p.group.d - w.c.block * ROWS, ROWS), wide = (d + 15) / 16;
-        for (uint32_t z = tid; z < ROWS * wide; z += threads) {
-            const uint32_t r = z % ROWS, x0 = z / ROWS * 4;
-            if (r >= rows) continue;
-            float m = -INFINITY, sum = 0.0f;
-            float4 o[4];
+        const uint32_t all_rows = min(q.news * p.group.d - w.c.block * ROWS, ROWS), n = last - first + 1;
+        const uint32_t step = min(all_rows, (room - 16 * threads - 4) / (2 * n));
+        for (uint32_t r0 = 0; r0 < all_rows; r0 += step) {
+            const uint32_t rows = min(step, all_rows - r0);
+            // Maxima and sums of the parts' rows, all loads at once; then what each part counts for, of each row. [part][row]
+            float *const factor = shared, *const sum = shared + n * rows;
+            for (uint32_t z = tid; z < n * rows; z += threads) {
+                const uint32_t k = z / rows;
+                const float *a = P::at(p.work, first + k, k == 0) + r0 + (z - k * rows);
+                factor[z] = __ldcg(a + P::TOP), sum[z] = __ldcg(a + P::SUM);
+            }
+            __syncthreads();
+            // `lanes` of a warp for each row, a part each.
+            uint32_t lanes = 1;
+            while (lanes < n && lanes < 32) lanes *= 2;
+            for (uint32_t z = tid; z < (rows * lanes + 31) / 32 * 32; z += threads) {
+                const uint32_t r = min(z / lanes, rows - 1), k0 = z & (lanes - 1);
+                const bool mine = z < rows * lanes;
+                float m = -INFINITY, all = 0.0f;
+                for (uint32_t k = k0; k < n; k += lanes) m = fmaxf(m, factor[k * rows + r]);
+                for (uint32_t x = 1; x < lanes; x *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+                const float ref = m == -INFINITY ? 0.0f : m;
+                for (uint32_t k = k0; k < n; k += lanes) all += sum[k * rows + r] * exp2_fast(factor[k * rows + r] - ref);
+                for (uint32_t x = 1; x < lanes; x *= 2) all += __shfl_xor_sync(0xffffffffu, all, x);
+                const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+                if (mine)
+                    for (uint32_t k = k0; k < n; k += lanes) factor[k * rows + r] = exp2_fast(factor[k * rows + r] - ref) * inv;
+                __syncwarp();
+            }
+            __syncthreads();
+            // A thread has four fours of columns of a row (32 bytes of the result, a sector) in every `groups`-th part; the groups' sums
+            // meet in shared memory.
+            const uint32_t wide = (d + 15) / 16, each = rows * wide, groups = max(1u, min(n, threads / each));
+            float4 *const met = reinterpret_cast<float4 *>(shared + (2 * n * rows + 3) / 4 * 4);
+            for (uint32_t z = tid; z < each * groups; z += threads) {
+                const uint32_t g = z / each, y0 = z - g * each, r = y0 % rows, x0 = y0 / rows * 4;
+                float4 o[4];
 #pragma unroll
-            for (uint32_t y = 0; y < 4; ++y) o[y] = make_float4(0, 0, 0, 0);
+                for (uint32_t y = 0; y < 4; ++y) o[y] = make_float4(0, 0, 0, 0);
 #pragma unroll 4
-            for (uint32_t k = first; k <= last; ++k) {
-                const float *a = P::at(p.work, k, k == first);
-                const float top = __ldcg(a + P::TOP + r), den = __ldcg(a + P::SUM + r);
-                float4 v[4];
+                for (uint32_t k = g; k < n; k += groups) {
+                    const float *a = P::at(p.work, first + k, k == 0);
+                    const float f = factor[k * rows + r];
+#pragma unroll
+                    for (uint32_t y = 0; y < 4; ++y) {
+                        if ((x0 + y) * 4 >= d) continue;
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(a + P::four(r0 + r, x0 + y)));
+                        o[y].x = fmaf(v.x, f, o[y].x), o[y].y = fmaf(v.y, f, o[y].y), o[y].z = fmaf(v.z, f, o[y].z), o[y].w = fmaf(v.w, f, o[y].w);
+                    }
+                }
+                if (groups > 1) {
+#pragma unroll
+                    for (uint32_t y = 0; y < 4; ++y) met[y * each * groups + z] = o[y];
+                    continue;
+                }
+                uint32_t token, head;
+                row_at(p, q, w.c.kv_head, w.c.block * ROWS + r0 + r, token, head);
+                uint16_t *out = p.out + ((size_t)token * p.n_heads + head) * d;
 #pragma unroll
                 for (uint32_t y = 0; y < 4; ++y)
-                    v[y] = (x0 + y) * 4 < d ? __ldcg(reinterpret_cast<const float4 *>(a + P::four(r, x0 + y))) : make_float4(0, 0, 0, 0);
-                const float all = fmaxf(m, top), ref = all == -INFINITY ? 0.0f : all;
-                const float f = exp2_fast(m - ref), g = exp2_fast(top - ref);
-                m = all;
-                sum = sum * f + den * g;
-#pragma unroll
-                for (uint32_t y = 0; y < 4; ++y) {
-                    o[y].x = o[y].x * f + v[y].x * g, o[y].y = o[y].y * f + v[y].y * g;
-                    o[y].z = o[y].z * f + v[y].z * g, o[y].w = o[y].w * f + v[y].w * g;
+                    if ((x0 + y) * 4 < d)
+                        *reinterpret_cast<uint2 *>(out + (x0 + y) * 4) = make_uint2(bf16_pair(o[y].x, o[y].y), bf16_pair(o[y].z, o[y].w));
+            }
+            if (groups > 1) {
+                __syncthreads();
+                for (uint32_t z = tid; z < each * 4; z += threads) {
+                    const uint32_t y = z / each, y0 = z - y * each, r = y0 % rows, x = y0 / rows * 4 + y;
+                    if (x * 4 >= d) continue;
+                    float4 o = make_float4(0, 0, 0, 0);
+                    for (uint32_t g = 0; g < groups; ++g) {
+                        const float4 v = met[(y * groups + g) * each + y0];
+                        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+                    }
+                    uint32_t token, head;
+                    row_at(p, q, w.c.kv_head, w.c.block * ROWS + r0 + r, token, head);
+                    *reinterpret_cast<uint2 *>(p.out + ((size_t)token * p.n_heads + head) * d + x * 4) = make_uint2(bf16_pair(o.x, o.y), bf16_pair(o.z, o.w));
                 }
             }
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            uint32_t token, head;
-            row_at(p, q, w.c.kv_head, w.c.block * ROWS + r, token, head);
-            uint16_t *out = p.out + ((size_t)token * p.n_heads + head) * d;
-#pragma unroll
-            for (uint32_t y = 0; y < 4; ++y)
-                if ((x0 + y) * 4 < d)
-                    *reinterpret_cast<uint2 *>(out + (x0 + y) * 4) = make_uint2(bf16_pair(o[y].x * inv, o[y].y * inv), bf16_pair(o[y].z * inv, o[y].w * inv));
+            __syncthreads();  // shared memory is read
         }
-        if (tid == 0) *P::counter(p, first) = 0;
+        if (tid == 0) *P::counter(p, first) = p.mark << 16;
     }
 }
 

@@ -21,11 +21,12 @@ namespace tessl {
 namespace attn {
 
 constexpr uint32_t kSplitRows = 16, kSplitUnit = 64, kStep = 16;
-constexpr uint32_t kSplitExtra = 16;  // a second part costs as much as 1024 keys
+constexpr uint32_t kSplitExtra = 9;
 
-template <int DP>
+/// BLOCKS: of an SM at a time.
+template <int DP, int BLOCKS>
 struct SplitCfg {
-    static constexpr uint32_t WARPS = 8, THREADS = WARPS * 32;
+    static constexpr uint32_t WARPS = 8 / BLOCKS, THREADS = WARPS * 32;
     static constexpr uint32_t CHUNKS = DP / 64;            // 64-column chunks of a row
     static constexpr uint32_t CHUNK = kStep * 128, TILE = CHUNKS * CHUNK;  // bytes
     static constexpr uint32_t SLOTS = 24576 / TILE;        // of a warp's ring: 12, 6, 4, 3
@@ -77,11 +78,11 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
 /// Byte offset of 16-byte piece c of row r of a tile of 16 rows: 64-column chunks one behind the other, 128-byte swizzle.
 __device__ __forceinline__ uint32_t piece_at(uint32_t r, uint32_t c) { return (c >> 3) * (kStep * 128) + r * 128 + (((c ^ r) & 7u) << 4); }
 
-template <int DP, bool TMA>
-__global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
+template <int DP, bool TMA, int BLOCKS>
+__global__ void __launch_bounds__(SplitCfg<DP, BLOCKS>::THREADS, BLOCKS)
     attn_paged_split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SplitParams sp)
 {
-    using C = SplitCfg<DP>;
+    using C = SplitCfg<DP, BLOCKS>;
     using P = Part<kSplitRows, DP>;
     constexpr uint32_t ROWS = kSplitRows, UNIT = kSplitUnit, SLOTS = C::SLOTS;
     asm volatile("griddepcontrol.launch_dependents;");
@@ -117,8 +118,7 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
     if (!line.start(p, blockIdx.x, shared, u, cur)) return;
     const uint32_t u_end = line.cut(blockIdx.x + 1);
     if (u >= u_end) return;
-    bool has[2] = {cur.u0 > 0, false};
-    if (tid == 0) pending[0] = Pending{cur, u - cur.u0};
+    bool has[2] = {false, false};
     uint32_t at = 0, phases = 0;  // the ring's next slot, the parity of each slot's next phase
 
     while (true) {
@@ -174,34 +174,46 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
                 cp_async_commit();
             }
         };
-        // Tiles K_0, V_0, K_1, ... of this warp. In flight: SLOTS of them. `holes`: for each of the steps that are on their way, the boxes
-        // (or a row: any) that are not there, two bits at step % 16.
+        // Tiles K_0, V_0, K_1, ... of this warp go into the ring one behind the other. `holes`: for each of the steps that are on their way,
+        // the boxes that are not there, two bits at step % 16 (rows: any row of any step).
         uint32_t holes = 0;
-        bool row_hole = false;  // rows: some row of some step is not there
-        auto note = [&](uint32_t j, const Where &w) {
-            if constexpr (TMA) {
-                const uint32_t gone = __ballot_sync(0xffffffffu, lane < boxes && w.page >= p.cache.num_pages);
-                holes = (holes & ~(3u << (j % 16 * 2))) | (gone << (j % 16 * 2));
-            } else {
-                row_hole |= __any_sync(0xffffffffu, w.page >= p.cache.num_pages && j < mine);
+        bool row_hole = false;
+        uint32_t issued = 0, done = 0, to = at;  // tiles asked for, tiles that have arrived, the slot of the next one
+        Where w = find(0), next = find(1);       // of the step whose tile is asked for next, and of the one behind it
+        auto feed = [&](uint32_t most) {
+#pragma unroll 2
+            for (uint32_t i = 0; i < most; ++i) {
+                if (issued < 2 * mine && issued - done < SLOTS) {
+                    const uint32_t j = issued / 2;
+                    if (issued % 2 == 0) {
+                        if constexpr (TMA) {
+                            const uint32_t gone = __ballot_sync(0xffffffffu, lane < boxes && w.page >= p.cache.num_pages);
+                            holes = (holes & ~(3u << (j % 16 * 2))) | (gone << (j % 16 * 2));
+                        } else {
+                            row_hole |= __any_sync(0xffffffffu, w.page >= p.cache.num_pages);
+                        }
+                        request(w, false, to);
+                    } else {
+                        request(w, true, to);
+                        w = next;
+                        next = find(j + 2);
+                    }
+                    ++issued;
+                    if (++to == SLOTS) to = 0;
+                } else if (!TMA) {
+                    cp_async_commit();
+                }
             }
         };
-        constexpr uint32_t H = SLOTS / 2;
-        constexpr bool ODD = SLOTS % 2;
-        Where first[H + ODD + 1];  // looked up together
-#pragma unroll
-        for (uint32_t j = 0; j < H + ODD + 1; ++j) first[j] = find(j);
-#pragma unroll
-        for (uint32_t j = 0; j < H + ODD; ++j) {
-            note(j, first[j]);
-            if (j < mine) request(first[j], false, (at + 2 * j) % SLOTS);
-            else if (!TMA) cp_async_commit();
-            if (j < H) {
-                if (j < mine) request(first[j], true, (at + 2 * j + 1) % SLOTS);
-                else if (!TMA) cp_async_commit();
-            }
+        // TMA: the first step only. 45 bytes a clock come out of the copy engine's requests, and a whole ring of every warp in front of the first
+        // step held that up by 4000 clocks; the rest is asked for behind it. Rows: a group for every slot (arrived() counts them).
+        feed(TMA ? 2 : SLOTS);
+
+        const bool whole = n_units == cur.units;
+        if (!whole) {
+            has[u0 == 0] = true;
+            if (tid == C::THREADS - 32) pending[u0 == 0] = Pending{cur, u - u0}, expect_parts<DP, ROWS>(p, line, u - u0);
         }
-        Where ahead = first[H], next = first[H + ODD];  // of step j + H: whose K, and V, are requested next; ODD: of the step whose V is
 
         // Q rows, zeros past the last row and column.
         for (uint32_t c = tid; c < ROWS * (DP / 8); c += C::THREADS) {
@@ -241,27 +253,27 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
             key_range(p, seq, i1, i1, lo_all, t);
             key_range(p, seq, i0, i0, t, hi_all);
         }
+        constexpr uint32_t REFILL = TMA ? 2 : 1;  // tiles asked for where one has been read, until the ring is full
         // The next tile in the ring has arrived: its slot.
         auto arrived = [&](uint32_t &slot) {
             slot = at;
-            bool ok = true;
             if constexpr (TMA) {
-                ok = __all_sync(0xffffffffu, q4k::mbar_wait(bars + 8 * at, (phases >> at) & 1u, abortp));
+                if (!__all_sync(0xffffffffu, q4k::mbar_wait(bars + 8 * at, (phases >> at) & 1u, abortp))) {
+                    if (lane == 0) *abortp = 1, *(volatile uint32_t *)p.status = (32u << 24) | blockIdx.x;
+                    return false;
+                }
                 phases ^= 1u << at;
-                if (!ok && lane == 0) *(volatile uint32_t *)p.status = (32u << 24) | blockIdx.x;
             } else {
                 cp_async_wait<SLOTS - 1>();
                 __syncwarp();
             }
             if (++at == SLOTS) at = 0;
-            return ok;
+            return true;
         };
-        uint32_t done = 0;  // tiles that have arrived
         for (uint32_t j = 0; j < mine; ++j) {
             const uint32_t key = key_of(j);
             uint32_t kt, vt;
             if (!arrived(kt)) break;
-            ++done;
             uint32_t gone = 0;  // bit t: key t is not there
             if constexpr (TMA) {
                 const uint32_t b = (holes >> (j % 16 * 2)) & 3u;
@@ -270,7 +282,7 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
                 const uint32_t k = key + (lane & 15u);
                 gone = __ballot_sync(0xffffffffu, k < key1 && (uint32_t)__ldcg(table + p.page.div(k)) >= p.cache.num_pages) & 0xffffu;
             }
-            float sc[2][4] = {};
+            float sc[2][4] = {}, odd[2][4] = {};  // two chains of MMAs for each eight keys
             const uint32_t ka = ring + kt * C::TILE;
 #pragma unroll
             for (uint32_t k = 0; k < DP / 16; ++k) {
@@ -283,24 +295,16 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
                 }
                 // keys 0-7 then 8-15, columns 16 k and 8 more
                 ldsm4(ka + piece_at((lane & 7u) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1u)), b);
-                mma_bf16(sc[0], a, b[0], b[1]);
-                mma_bf16(sc[1], a, b[2], b[3]);
+                mma_bf16(k % 2 ? odd[0] : sc[0], a, b[0], b[1]);
+                mma_bf16(k % 2 ? odd[1] : sc[1], a, b[2], b[3]);
             }
             __syncwarp();  // the tile is read
-            if (ODD) {
-                if (j + H < mine) request(ahead, true, kt);
-                else if (!TMA) cp_async_commit();
-                ahead = next;
-                next = find(j + H + 2);
-            } else {
-                if (j + H < mine) note(j + H, ahead), request(ahead, false, kt);
-                else if (!TMA) cp_async_commit();
-                next = find(j + H + 1);
-            }
+            ++done;
+            feed(REFILL);
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) sc[n][x] *= p.scale_log2;
+                for (int x = 0; x < 4; ++x) sc[n][x] = (sc[n][x] + odd[n][x]) * p.scale_log2;
             if (gone || key < lo_all || key + kStep > min(hi_all, key1)) {
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
@@ -335,7 +339,6 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
             }
             const uint32_t pf[4] = {bf16_pair(sc[0][0], sc[0][1]), bf16_pair(sc[0][2], sc[0][3]), bf16_pair(sc[1][0], sc[1][1]), bf16_pair(sc[1][2], sc[1][3])};
             if (!arrived(vt)) break;
-            ++done;
             const uint32_t va = ring + vt * C::TILE;
             if (TMA && key + kStep > seq.keys) {  // slots behind the sequence may hold anything: no values
                 const uint32_t first = seq.keys - key;
@@ -353,21 +356,14 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
                 mma_bf16(o[2 * n + 1], pf, b[2], b[3]);
             }
             __syncwarp();  // the tile is read
-            if (ODD) {
-                if (j + H + 1 < mine) note(j + H + 1, ahead), request(ahead, false, vt);
-                else if (!TMA) cp_async_commit();
-            } else {
-                if (j + H < mine) request(ahead, true, vt);
-                else if (!TMA) cp_async_commit();
-                ahead = next;
-            }
+            ++done;
+            feed(REFILL);
         }
         if constexpr (TMA) {
-            if (*abortp && done < 2 * mine) {  // what is on its way must land before the block ends
-                const uint32_t on_way = min(2 * mine - done, SLOTS);
+            if (*abortp) {  // what is on its way must land before the block ends
                 const long long t0 = clock64();
-                for (uint32_t k = 0; k < on_way; ++k) {
-                    const uint32_t slot = (at + k) % SLOTS;
+                for (uint32_t k = done; k < issued; ++k) {
+                    const uint32_t slot = (to + SLOTS - (issued - k)) % SLOTS;
                     while (!q4k::mbar_try(bars + 8 * slot, (phases >> slot) & 1u))
                         if (clock64() - t0 > 20000000ll) break;
                 }
@@ -398,7 +394,6 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
                     make_float2(o[n][2 * h] * f, o[n][2 * h + 1] * f);
         }
         __syncthreads();
-        const bool whole = n_units == cur.units;
         float *part = P::at(p.work, blockIdx.x, u0 == 0);
         for (uint32_t c = tid; c < min(ROWS, rows - row0) * (DP / 4); c += C::THREADS) {
             const uint32_t r = c / (DP / 4), x = c % (DP / 4);
@@ -427,10 +422,6 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
                 if (x == 0) part[P::TOP + r] = t, part[P::SUM + r] = den;
             }
         }
-        if (!whole && u0 == 0) {
-            has[1] = true;
-            if (tid == 0) pending[1] = Pending{cur, u};
-        }
         u += line.places(n_units);
         if (u >= u_end) break;
         L::next(p, cur);
@@ -438,7 +429,7 @@ __global__ void __launch_bounds__(SplitCfg<DP>::THREADS, 1)
         __syncthreads();              // rings, Q and ml are read
     }
     __syncthreads();
-    finish_parts<DP, ROWS>(p, line, pending, has, C::THREADS, came);
+    finish_parts<DP, ROWS>(p, line, pending, has, C::THREADS, came, reinterpret_cast<float *>(smem), C::WARPS * C::RING / 4);
 }
 
 }  // namespace attn

@@ -240,14 +240,9 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
     L line;
     Cursor cur;
     uint32_t u = 0, u_end = 0;
-    bool has[2] = {false, false};
     if (line.start(p, blockIdx.x, *reinterpret_cast<typename L::Shared *>(smem_raw + C::Q_BYTES), u, cur)) u_end = line.cut(blockIdx.x + 1);
     const uint32_t u_start = u;
-    if (tid == 0) pending[1].from = ~0u;
-    if (u < u_end) {
-        has[0] = cur.u0 > 0;
-        if (tid == 0) pending[0] = Pending{cur, u - cur.u0};
-    }
+    if (tid < 2) pending[tid].from = ~0u;
     fence_async_smem();  // the ring's next writer is the copy engine
     __syncthreads();
     // The item at the cursor, as every role sees it: n tiles of keys from k0 on, in `steps` steps.
@@ -320,6 +315,8 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                 for (uint32_t i = 0; i < A; ++i) pk[i] = pk[i + 1], sk[i] = sk[i + 1];
                 pk[A] = np, sk[A] = ns;
             }
+            if (n_units != cur.units && lane == 0)
+                pending[cur.u0 == 0] = Pending{cur, u - cur.u0}, expect_parts<DP, C::ROWS>(p, line, u - cur.u0);
             u += line.places(n_units);
             if (u < u_end) L::next(p, cur);
         }
@@ -591,7 +588,6 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                 }
             }
             const bool whole = n_units == cur.units;
-            if (!whole && cur.u0 == 0 && tid == 0) pending[1] = Pending{cur, u};
             float *part = P::at(p.work, blockIdx.x, cur.u0 == 0);
             tiles += 2 * n;
             u += line.places(n_units);
@@ -668,8 +664,9 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(pf::kTmemCols) : "memory");
     }
     if (*abortp || u_start >= u_end) return;
-    has[1] = pending[1].from != ~0u;
-    finish_parts<DP, C::ROWS>(p, line, pending, has, C::THREADS, reinterpret_cast<volatile uint32_t *>(smem_raw + C::SMEM - 16));
+    const bool has[2] = {pending[0].from != ~0u, pending[1].from != ~0u};
+    finish_parts<DP, C::ROWS>(p, line, pending, has, C::THREADS, reinterpret_cast<volatile uint32_t *>(smem_raw + C::SMEM - 16),
+                         reinterpret_cast<float *>(smem_raw), (C::Q_BYTES + C::SLOTS * C::SLOT) / 4);
 }
 
 }  // namespace attn
