@@ -344,6 +344,91 @@ __device__ __forceinline__ void row_at(const Params &p, const Seq &q, uint32_t k
     token += q.row0;
 }
 
+// Values that are not finite, of keys that some rows of an item see and others do not: a weight of 0 times such a value is NaN, so the
+// kernels make zeros of them in shared memory and note that they did. A block that has done so adds them, at its end, to the rows that see
+// them. All rows of the item see [lo_all, hi_all).
+
+__device__ __forceinline__ bool some_unseen(uint32_t key, uint32_t lo_all, uint32_t hi_all) { return key < lo_all || key >= hi_all; }
+/// The same of any of the sequence's keys in [key, key + n).
+__device__ __forceinline__ bool some_unseen(const Seq &q, uint32_t key, uint32_t n, uint32_t lo_all, uint32_t hi_all)
+{
+    return key < lo_all || min(key + n, q.keys) > hi_all;
+}
+/// N times eight bf16 values at shared-memory addresses at(0) .., those that are not finite made zero: whether there were any.
+template <int N, typename F>
+__device__ __forceinline__ bool make_finite(F at)
+{
+    uint32_t w[N][4], bad = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[k][0]), "=r"(w[k][1]), "=r"(w[k][2]), "=r"(w[k][3]) : "r"(at(k)) : "memory");
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad |= (w[k][i] & 0x7f807f80u) + 0x00800080u;  // an exponent of ones carries into the sign's place
+    if (!(bad & 0x80008000u)) return false;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if ((w[k][i] & 0x7f80u) == 0x7f80u) w[k][i] &= 0xffff0000u;
+            if ((w[k][i] & 0x7f800000u) == 0x7f800000u) w[k][i] &= 0xffffu;
+        }
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at(k)), "r"(w[k][0]), "r"(w[k][1]), "r"(w[k][2]), "r"(w[k][3]) : "memory");
+    }
+    return true;
+}
+/// The block's items once more. All threads, behind a barrier. (Not inlined, the call's conventions cost a kernel that never came here
+/// 12 us of 119.)
+template <uint32_t DP, uint32_t ROWS, uint32_t UNIT, typename L>
+__device__ __forceinline__ void add_not_finite(const Params &p, typename L::Shared &sh, uint32_t threads)
+{
+    using P = Part<ROWS, DP>;
+    L line;
+    Cursor cur;
+    uint32_t u;
+    if (!line.start(p, blockIdx.x, sh, u, cur)) return;
+    const uint32_t u_end = line.cut(blockIdx.x + 1), d = p.cache.head_dim;
+    while (u < u_end) {
+        const Seq &q = cur.seq;
+        const uint32_t n_units = line.units_to(cur, u, u_end), row0 = cur.block * ROWS, end = min(row0 + ROWS, q.news * p.group.d);
+        const uint32_t i0 = p.group.div(row0), i1 = p.group.div(end - 1);
+        uint32_t lo, hi, lo_all, hi_all, t;
+        key_range(p, q, i0, i1, lo, hi), key_range(p, q, i1, i1, lo_all, t), key_range(p, q, i0, i0, t, hi_all);
+        const uint32_t k0 = (cur.first + cur.u0) * UNIT, k1 = min(k0 + n_units * UNIT, hi);
+        float *part = P::at(p.work, blockIdx.x, cur.u0 == 0);
+        for (uint32_t key = max(k0, lo); key < k1; ++key) {
+            if (!some_unseen(key, lo_all, hi_all)) {
+                key = min(hi_all, k1) - 1;
+                continue;
+            }
+            const uint32_t page = (uint32_t)__ldcg(p.seqs.table + (size_t)q.index * p.seqs.max_pages + p.page.div(key));
+            if (page >= p.cache.num_pages) continue;
+            const uint16_t *v = p.cache.v + page * p.cache.page_stride + (uint64_t)p.page.mod(key) * p.cache.token_stride +
+                                (uint64_t)cur.kv_head * p.cache.head_stride;
+            for (uint32_t c = threadIdx.x; c < d; c += threads) {
+                const uint32_t bits = __ldcg(v + c);
+                if ((bits & 0x7f80u) != 0x7f80u) continue;
+                const float x = __uint_as_float(bits << 16);
+                for (uint32_t r = row0; r < end; ++r) {
+                    uint32_t token = p.group.div(r), head, lo_r, hi_r;
+                    key_range(p, q, token, token, lo_r, hi_r);
+                    if (key < lo_r || key >= hi_r) continue;
+                    row_at(p, q, cur.kv_head, r, token, head);
+                    if (n_units == cur.units) {
+                        uint16_t *at = p.out + ((size_t)token * p.n_heads + head) * d + c;
+                        *at = (uint16_t)bf16_pair(__uint_as_float((uint32_t)*at << 16) + x, 0.0f);
+                    } else {
+                        part[P::four(r - row0, c / 4) + c % 4] += x;
+                    }
+                }
+            }
+        }
+        u += line.places(n_units);
+        if (u < u_end) L::next(p, cur);
+    }
+}
+
 /// Before a barrier in front of finish_parts, by one thread, for each item (where it begins on the line) of which the block has a part: a counter that does not hold a number of
 /// this call's own and a count holds what another call or nobody has put there, and is given the number and a count of 0 by the first block
 /// to see that. Whoever has added up puts the count back to 0, for a replay of this call has the same number.

@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(SplitCfg<DP, BLOCKS>::THREADS, BLOCKS)
     using L = Line<ROWS, UNIT, C::THREADS, kSplitExtra>;
     __shared__ typename L::Shared shared;
     __shared__ Pending pending[2];
-    __shared__ int abort_flag;
+    __shared__ int abort_flag, made_finite;
     __shared__ uint32_t came[2];
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t ring = q4k::smem_u32(smem) + warp * C::RING, q_smem = q4k::smem_u32(smem) + C::WARPS * C::RING;
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(SplitCfg<DP, BLOCKS>::THREADS, BLOCKS)
     const uint32_t bars = q_smem + C::Q_BYTES + C::ML_BYTES + warp * SLOTS * 8;
     const uint32_t d = p.cache.head_dim, pieces = d / 8;
     volatile int *abortp = &abort_flag;
-    if (tid == 0) abort_flag = 0;
+    if (tid == 0) abort_flag = 0, made_finite = 0;
     if (TMA && lane == 0) {
         for (uint32_t s = 0; s < SLOTS; ++s) q4k::mbar_init(bars + 8 * s, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -340,11 +340,14 @@ __global__ void __launch_bounds__(SplitCfg<DP, BLOCKS>::THREADS, BLOCKS)
             const uint32_t pf[4] = {bf16_pair(sc[0][0], sc[0][1]), bf16_pair(sc[0][2], sc[0][3]), bf16_pair(sc[1][0], sc[1][1]), bf16_pair(sc[1][2], sc[1][3])};
             if (!arrived(vt)) break;
             const uint32_t va = ring + vt * C::TILE;
-            if (TMA && key + kStep > seq.keys) {  // slots behind the sequence may hold anything: no values
-                const uint32_t first = seq.keys - key;
-                for (uint32_t c = lane + first * (DP / 8); c < kStep * (DP / 8); c += 32)
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(va + piece_at(c / (DP / 8), c % (DP / 8))), "r"(0) : "memory");
-                fence_async_smem();  // the slot's next writer is the copy engine
+            if ((TMA && key + kStep > seq.keys) || some_unseen(seq, key, kStep, lo_all, hi_all)) {
+#pragma unroll 1
+                for (uint32_t c = lane; c < kStep * (DP / 8); c += 32) {
+                    const uint32_t k = key + c / (DP / 8), x = va + piece_at(c / (DP / 8), c % (DP / 8));
+                    if (k >= seq.keys) asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(x), "r"(0) : "memory");  // may hold anything: no values
+                    else if (some_unseen(k, lo_all, hi_all) && make_finite<1>([&](int) { return x; })) *(volatile int *)&made_finite = 1;
+                }
+                if (TMA) fence_async_smem();  // the slot's next writer is the copy engine
                 __syncwarp();
             }
 #pragma unroll
@@ -429,6 +432,10 @@ __global__ void __launch_bounds__(SplitCfg<DP, BLOCKS>::THREADS, BLOCKS)
         __syncthreads();              // rings, Q and ml are read
     }
     __syncthreads();
+    if (made_finite) {
+        add_not_finite<DP, ROWS, UNIT, L>(p, shared, C::THREADS);
+        __syncthreads();
+    }
     finish_parts<DP, ROWS>(p, line, pending, has, C::THREADS, came, reinterpret_cast<float *>(smem), C::WARPS * C::RING / 4);
 }
 

@@ -13,10 +13,9 @@
 // K and V come by TMA, page by page, as 64-column chunks of 128 keys with the 128-byte swizzle: K is the K-major B operand of
 // the first product, V the MN-major B operand of the second. Pages outside the cache and keys past the sequence's last page
 // arrive as zeros; slots of the last page behind the sequence may hold anything, so their rows of V are zeroed in shared
-// memory before the product (0 times NaN).
+// memory before the product (0 times NaN), as are values of V that are not finite and that some rows see and others do not.
 //
-// Rounding of the weights: see attn_paged_split.cuh. A value of V that is not finite reaches the rows that see its token; in the tiles
-// in which some rows see the token and others do not, it reaches those too (0 times it).
+// Rounding of the weights: see attn_paged_split.cuh.
 //
 // Roles: eight warps softmax, Q and the results, one warp TMA, a warp for each row tile MMA issue. Every wait is bounded; on a
 // timeout the status word is set and all roles fall through to the end.
@@ -196,6 +195,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
     const uint32_t q_smem = q4k::smem_u32(smem_raw), ring = q_smem + C::Q_BYTES, bar0 = ring + C::SLOTS * C::SLOT + C::X_BYTES;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem_raw + C::SMEM - 32);
     volatile int *abortp = reinterpret_cast<volatile int *>(smem_raw + C::SMEM - 24);
+    volatile int *made_finite = reinterpret_cast<volatile int *>(smem_raw + C::SMEM - 20);
     Pending *pending = reinterpret_cast<Pending *>(smem_raw + C::SMEM - 32 - 2 * sizeof(Pending));  // items of which this block has a part
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     auto slot_full = [&](uint32_t s) { return bar0 + 8 * s; };
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
             mbar_init(q_full(lane), 4 * C::TPR), mbar_init(o_free(lane), 4 * C::TPR);
         }
         if (lane == 0) {
-            *abortp = 0;
+            *abortp = 0, *made_finite = 0;
             mbar_init(done, NT);
             asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
@@ -496,6 +496,12 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                     key_range(p, cur.seq, i, i, lo_r, hi_r);
                 }
                 const uint32_t lo_all = __shfl_sync(0xffffffffu, lo_r, 31), hi_all = __shfl_sync(0xffffffffu, hi_r, 0);
+                uint32_t lo_item, hi_item;  // what all rows of the item see: its row tiles read the same V
+                {
+                    uint32_t x;
+                    const uint32_t i0 = p.group.div(row0), i1 = p.group.div(min(row0 + C::ROWS, rows) - 1);
+                    key_range(p, cur.seq, i1, i1, lo_item, x), key_range(p, cur.seq, i0, i0, x, hi_item);
+                }
                 const int32_t *table = p.seqs.table + (size_t)cur.seq.index * p.seqs.max_pages;
                 auto page_of = [&](uint32_t key) { return key < cur.seq.keys ? (uint32_t)__ldcg(table + p.page.div(key)) : 0u; };
                 bool any_hole = false;  // a page of the item is not there: its tiles look at theirs
@@ -558,18 +564,31 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
                         w[y] = bf16_pair(a, b);
                     }
                     tmem_store32(s_tmem, w);
-                    if (key + 64 > cur.seq.keys) {  // slots behind the sequence: no values
-                        const uint32_t j = i / C::SPK, first = i % C::SPK * C::SK + 64 * half;  // the tile of V, this thread's first row of it
-                        for (uint32_t y = 0; y < C::SPT; ++y) {
-                            const uint32_t z = (tiles + v_place(j)) * C::SPT + y, slot = ring + z % C::SLOTS * C::SLOT;
-                            if (!wait(slot_full(z % C::SLOTS), (z / C::SLOTS) & 1u, 8, j)) break;
-                            if (r / 64 == first / 64 && key + r % 64 >= cur.seq.keys)
-                                for (uint32_t q = 0; q < C::CPS * 8; ++q)
-                                    asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(slot + q / 8 * C::CHUNK + r * 128 + (q % 8) * 16), "r"(0) : "memory");
+                    const uint32_t step = k0 + i * C::SK;
+                    if (step + C::SK > cur.seq.keys || some_unseen(cur.seq, step, C::SK, lo_item, hi_item)) {
+                        // Two threads for a row of V. Slots behind the sequence: no values.
+                        const uint32_t x = half * 128 + r, of = x % C::SK, j = i / C::SPK, v_row = i % C::SPK * C::SK + of;
+                        const bool past = step + of >= cur.seq.keys, look = some_unseen(step + of, lo_item, hi_item);
+                        if (__any_sync(0xffffffffu, past || look)) {
+#pragma unroll 1
+                            for (uint32_t y = 0; y < C::SPT; ++y) {
+                                const uint32_t z = (tiles + v_place(j)) * C::SPT + y, at = ring + z % C::SLOTS * C::SLOT + v_row * 128;
+                                if (!wait(slot_full(z % C::SLOTS), (z / C::SLOTS) & 1u, 8, j)) break;
+#pragma unroll 1
+                                for (uint32_t c = 0; c < C::CPS; ++c) {
+                                    auto piece = [&](uint32_t k) { return at + c * C::CHUNK + (((x / C::SK * 4 + k) ^ (v_row & 7u)) << 4); };  // lanes on different banks
+                                    if (past) {
+#pragma unroll
+                                        for (uint32_t k = 0; k < 4; ++k) asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(piece(k)), "r"(0) : "memory");
+                                    } else if (look && make_finite<4>(piece)) {
+                                        *made_finite = 1;
+                                    }
+                                }
+                            }
+                            fence_async_smem();
+                            __syncwarp();
+                            if (!ok) break;
                         }
-                        fence_async_smem();
-                        __syncwarp();
-                        if (!ok) break;
                     }
                     tmem_store_wait();
                     pf::tcgen05_fence_before();
@@ -664,6 +683,10 @@ __global__ void __launch_bounds__(TileCfg<DP>::THREADS, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(pf::kTmemCols) : "memory");
     }
     if (*abortp || u_start >= u_end) return;
+    if (*made_finite) {
+        add_not_finite<DP, C::ROWS, kTileKeys, L>(p, *reinterpret_cast<typename L::Shared *>(smem_raw + C::Q_BYTES), C::THREADS);
+        __syncthreads();
+    }
     const bool has[2] = {pending[0].from != ~0u, pending[1].from != ~0u};
     finish_parts<DP, C::ROWS>(p, line, pending, has, C::THREADS, reinterpret_cast<volatile uint32_t *>(smem_raw + C::SMEM - 16),
                          reinterpret_cast<float *>(smem_raw), (C::Q_BYTES + C::SLOTS * C::SLOT) / 4);
