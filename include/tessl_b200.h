@@ -522,7 +522,10 @@ TESSL_API uint64_t tessl_attn_paged_workspace_bytes(TesslRuntime *rt, uint32_t t
  * [total_new, n_heads, head_dim] with rows q_stride elements apart (0 = one behind
  * the other, else a multiple of 8), out bf16 [total_new, n_heads, head_dim]: what
  * the output projection reads. Scores, softmax and sums in f32; the weights p are
- * rounded to bf16 for the product with v, after the sum over them was taken. */
+ * rounded to bf16 for the product with v, after the sum over them was taken. An
+ * infinity or NaN in v of a token reaches the rows that see it, in its column, a
+ * score that is +infinity or NaN makes its row NaN; rows that do not see a token
+ * are as if it were not there. A call of more than 2^32 units of 16 rows by 64 keys is refused. */
 TESSL_API int32_t tessl_attn_paged(TesslRuntime *rt, TesslBuf q, const TesslPagedKv *cache, const TesslPagedSeqs *seqs,
                                    TesslBuf out, TesslBuf workspace, uint32_t total_new, uint32_t n_heads,
                                    uint32_t q_stride, float scale, uint32_t causal, uint32_t window, char *err,

@@ -31,13 +31,17 @@ auto with_dim(uint32_t head_dim, F f)
 /// swizzle's groups of eight rows.
 uint32_t box_of(uint32_t page_size, uint32_t most) { return std::min(page_size & (0u - page_size), most); }
 
-/// Whether a call of these sizes goes to the tensor-core tiles: enough rows for each key head of a sequence to fill some of a tile.
+/// Whether a call of these sizes goes to the tensor-core tiles: more than 32 rows for each key head of a sequence, on average. Eight
+/// sequences of up to 8000 keys, 32 heads of 128 on 8, with the kernel for few rows and with the tiles: 16 rows 56 and 60 us, 24 rows 66 and
+/// 60 us, 48 rows 83 and 61 us; one sequence: 32 rows 25 and 29 us, 64 rows 42 and 39 us; four sequences of wide heads: 32 rows 51 and 50 us.
 bool wants_tiles(const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t group)
 {
     return seqs.q_starts.ptr && cache.num_pages > 0 && cache.page_size % 8 == 0 && elems(total_new, group) > 32ull * seqs.num_seqs;
 }
 
-/// Blocks of the split kernel on an SM.
+/// Blocks of the split kernel on an SM: two, of half the warps each, where there are more items than SMs, so that one reads while the other
+/// starts or ends an item. With one and with two, heads as above, a token each: 64 sequences of up to 1000 keys 58 and 49 us, 24 of up to
+/// 6000 keys 87 and 80 us, 12 of up to 6000 keys 51 and 50 us, 8 of up to 500 keys 11 and 16 us, one of 130001 keys 103 and 107 us.
 uint32_t split_blocks(const TesslRuntime *rt, const TesslPagedKv &cache, const TesslPagedSeqs &seqs)
 {
     return elems(seqs.num_seqs, cache.n_kv_heads) > (uint64_t)rt->sm_count ? 2 : 1;

@@ -7,7 +7,7 @@
 // sequences, every block reads the same number of keys. The lengths are on the device, so the blocks work the cuts out
 // themselves. A block that has an item to itself writes its rows; the parts of an item that a cut divides go to the workspace,
 // two at most per block (the end of one item, the start of another). A block counts its parts in when it is done: the last one of an
-// item to come adds the parts up, in the order of the keys, the same sums on every run. (A second launch for the sums took 9 us
+// item to come adds the parts up, in an order that their number alone decides: the same sums on every run. (A second launch took 9 us
 // of the 18 of a token over 777 keys, and 21 of 74 of ragged chunks.)
 #pragma once
 #include "paged_common.cuh"
@@ -238,7 +238,7 @@ struct Line {
         const uint32_t total = whole ? items : units;
         per_head = whole ? all.blocks : all.units;
         span = total, cuts = min(p.parts, total);
-        // A few items of the same length: no block has parts of two.
+        // A few items of the same length: no block has parts of two, which cost a token over 3000 keys 20 us instead of 14.5.
         if (!whole && all.most * all.blocks == all.units && items <= p.parts) {
             const uint32_t k = min(p.parts / items, all.most);
             if ((all.most + k - 1) / k <= units / p.parts + EXTRA / 2) span = all.most, cuts = k;
