@@ -4,8 +4,8 @@ Three kinds of case:
 
 * ``layers``: one pass of `m` token rows through the quantized part of a few transformer layers (embedding gather,
   then per layer norm, q/k/v projection, output projection with the residual, norm, gated MLP with the residual).
-  m = 1 is single-stream decode, 2..8 batched decode, more a prompt. Attention itself is not part of the library, so
-  its output is an input here. A program that decodes in a loop keeps the step in a CUDA graph (``graph``) or makes
+  m = 1 is single-stream decode, 2..8 batched decode, more a prompt. These are the projections' passes: attention's
+  output is an input here. A program that decodes in a loop keeps the step in a CUDA graph (``graph``) or makes
   the calls one by one in encode-only mode.
 * ``q4``: a single 4-bit projection, routed by m as `Q4Weight.matmul` does: GEMV, small-batch GEMM, prefill GEMM.
 * ``q8`` / ``q8_signed``: a single 8-bit projection in MLX's format (m <= 8) or with signed codes and f32 tables (m = 1).
