@@ -143,7 +143,7 @@ Result attn_paged(TesslRuntime *rt, const TesslBuf &q, const TesslPagedKv &cache
     const char *what = "attn_paged";
     Params p{};
     TESSL_TRY(attn_params(cache, seqs, total_new, n_heads, what, &p));
-    if (!std::isfinite(scale)) return fmt("%s: scale is not finite", what);
+    if (!std::isfinite(scale * 1.4426950408889634f)) return fmt("%s: scale is not finite, or too large", what);
     if (window && !causal) return fmt("%s: a window needs causal attention", what);
     const uint64_t width = elems(n_heads, cache.head_dim);
     uint32_t out_stride = 0;
@@ -166,6 +166,7 @@ Result attn_paged(TesslRuntime *rt, const TesslBuf &q, const TesslPagedKv &cache
     if (total_new == 0 || seqs.num_seqs == 0) return ok();
     p.q = static_cast<const uint16_t *>(q.ptr), p.out = static_cast<uint16_t *>(out.ptr), p.work = static_cast<float *>(workspace.ptr);
     p.q_stride = q_stride;
+    if (cache.num_pages == 0) p.cache.k = p.cache.v = static_cast<uint16_t *>(q.ptr);  // copies of no bytes still name an address
     p.causal = causal, p.window = window, p.status = rt->status_dev;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.mark = next_mark(rt);

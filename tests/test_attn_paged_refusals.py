@@ -193,7 +193,7 @@ def test_attention_refuses(host_rt):
     cache, seqs, total = paged()
     for heads in (0, 3):
         refused("n_heads %d" % heads, call_attn, host_rt, cache, seqs, total, heads=heads)
-    for s in (float("nan"), float("inf")):
+    for s in (float("nan"), float("inf"), -3e38):
         refused("scale", call_attn, host_rt, cache, seqs, total, scale=s)
     refused("window needs causal", call_attn, host_rt, cache, seqs, total, causal=False, window=4)
     refused("attn_paged q", call_attn, host_rt, cache, seqs, total, q=buf(3 * 4 * 64 * 2 - 2))

@@ -134,3 +134,36 @@ def test_a_cache_of_more_than_2_32_values(rt, major, news):
     live = small.k.reshape(-1, each) != 0x7FC1
     assert np.array_equal(got[live], small.k.reshape(-1, each)[live])
     assert np.isfinite(f64(got[live])).all()
+
+
+@pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("pages,width", [(0, 3), (3, 0), (0, 0)])
+def test_no_pages_or_no_table(rt, pages, width, new):
+    b = Batch(90, [70, 20], [new, new], 2, 2, 64, 16).upload(rt)
+    none = nn.GpuBuffer(0, 0)
+    cache = nn.PagedKv(b.b_k if pages else none, b.b_v if pages else none, pages, 16, 2, 64)
+    seqs = nn.PagedSeqs(b.seqs.page_table if width else none, b.seqs.kv_lens, b.seqs.q_starts, 2, width)
+    work = rt.alloc_buffer(nn.attn_paged_workspace_bytes(rt, b.total, b.heads, cache, seqs))
+    nn.attn_paged(rt, b.b_q, cache, seqs, b.out.view(0, b.q.size * 2), work, b.total, b.heads, 0.125)
+    kv = rt.buffer_from(bf16(np.ones((b.total, 2, 64))))
+    nn.kv_append_paged(rt, None, kv, rt.buffer_from(bf16(np.ones((b.total, 2, 64)))), None, cache, seqs, None, None, b.total, 0, in_as_bf16=True)
+    rt.synchronize()
+    got = b.out.read(np.uint16, b.q.size + 64)
+    if pages == 0 or width == 0:
+        assert (got[:b.q.size] & 0x7FFF == 0).all() and (got[b.q.size:] == SENTINEL16).all()
+
+
+def test_offsets_that_go_back_and_forth_count_to_an_end(rt):
+    """Descending offsets may not be given; the work that they add up to is more than the kernels count, and nothing is done."""
+    n, tokens, page = 1200, 1024, 1 << 20
+    cache = nn.PagedKv(rt.buffer_from(np.zeros(page * 8, np.uint16)), rt.buffer_from(np.zeros(page * 8, np.uint16)), 1, page, 1, 8)
+    starts = np.zeros(n + 1, np.int32)
+    starts[1::2] = tokens
+    seqs = nn.PagedSeqs(rt.buffer_from(np.zeros(n, np.int32)), rt.buffer_from(np.full(n, page, np.int32)), rt.buffer_from(starts), n, 1)
+    q = rt.buffer_from(np.zeros(tokens * 16 * 8, np.uint16))
+    out = rt.buffer_from(np.full(tokens * 16 * 8, SENTINEL16, np.uint16))
+    work = rt.alloc_buffer(nn.attn_paged_workspace_bytes(rt, tokens, 16, cache, seqs))
+    nn.attn_paged(rt, q, cache, seqs, out, work, tokens, 16, 0.3, causal=False)
+    rt.synchronize()
+    assert not rt.is_poisoned()
+    assert (out.read(np.uint16, tokens * 16 * 8) == SENTINEL16).all()
