@@ -461,15 +461,15 @@ __device__ void finish_parts(const Params &p, const L &l, const Pending *pending
     if (!has[0] && !has[1]) return;
     const uint32_t tid = threadIdx.x, d = p.cache.head_dim;
     if (tid == 0) {
-        __threadfence();  // the block's parts, behind the barrier that all have passed
+        // Releases the block's parts, behind the barrier that all have passed, and acquires those of the blocks before.
         unsigned long long old[2];
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i)
-            if (has[i]) old[i] = atomicAdd(P::counter(p, l.part_of(pending[i].from)), 1ull);
+            if (has[i])
+                asm volatile("atom.acq_rel.gpu.global.add.u64 %0, [%1], 1;" : "=l"(old[i]) : "l"(P::counter(p, l.part_of(pending[i].from))) : "memory");
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i)
             if (has[i]) came[i] = (uint32_t)(old[i] & 0xffffu) + 1;
-        __threadfence();
     }
     __syncthreads();
     for (uint32_t i = 0; i < 2; ++i) {

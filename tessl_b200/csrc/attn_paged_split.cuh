@@ -257,6 +257,7 @@ __global__ void __launch_bounds__(SplitCfg<DP, BLOCKS>::THREADS, BLOCKS)
             key_range(p, seq, i1, i1, lo_all, t);
             key_range(p, seq, i0, i0, t, hi_all);
         }
+        const uint32_t edge_hi = min(hi_all, key1);
         constexpr uint32_t REFILL = TMA ? 2 : 1;  // tiles asked for where one has been read, until the ring is full
         // The next tile in the ring has arrived: its slot.
         auto arrived = [&](uint32_t &slot) {
@@ -309,7 +310,8 @@ __global__ void __launch_bounds__(SplitCfg<DP, BLOCKS>::THREADS, BLOCKS)
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) sc[n][x] = (sc[n][x] + odd[n][x]) * p.scale_log2;
-            if (gone || key < lo_all || key + kStep > min(hi_all, key1)) {
+            const bool edge = key < lo_all || key + kStep > edge_hi;  // keys that not all rows see, or behind the sequence
+            if (gone || edge) {
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -344,7 +346,7 @@ __global__ void __launch_bounds__(SplitCfg<DP, BLOCKS>::THREADS, BLOCKS)
             const uint32_t pf[4] = {bf16_pair(sc[0][0], sc[0][1]), bf16_pair(sc[0][2], sc[0][3]), bf16_pair(sc[1][0], sc[1][1]), bf16_pair(sc[1][2], sc[1][3])};
             if (!arrived(vt)) break;
             const uint32_t va = ring + vt * C::TILE;
-            if ((TMA && key + kStep > seq.keys) || some_unseen(seq, key, kStep, lo_all, hi_all)) {
+            if (edge && ((TMA && key + kStep > seq.keys) || some_unseen(seq, key, kStep, lo_all, hi_all))) {
 #pragma unroll 1
                 for (uint32_t c = lane; c < kStep * (DP / 8); c += 32) {
                     const uint32_t k = key + c / (DP / 8), x = va + piece_at(c / (DP / 8), c % (DP / 8));
