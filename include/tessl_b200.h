@@ -396,9 +396,8 @@ TESSL_API int32_t tessl_qwen35_add_rms_norm(TesslRuntime *rt, TesslBuf y, TesslB
 
 /* What lies between a layer's q/k/v projection and its output projection: rotary
  * positions, a paged cache of keys and values, and attention over it. The
- * reference has these as kernels of its Metal tower (its rope, kv_store and
- * flash_attn families); the entries here are this library's own, in its
- * conventions: device buffers with capacities, everything that the host can see
+ * reference has kernels for these in its own model; the entries here are this
+ * library's own, in its conventions: device buffers with capacities, everything that the host can see
  * checked before any launch, nothing allocated, all of it safe to capture.
  * What only the device can see (lengths, offsets, page ids) is checked by the
  * kernels, which leave out what points outside. */
