@@ -113,15 +113,10 @@ struct Pending {
 /// cutting items would cost more than it gives, whole items. EXTRA: what an item's second part costs, in units.
 template <uint32_t ROWS, uint32_t UNIT, uint32_t THREADS, uint32_t EXTRA>
 struct Line {
-    /// Of some sequences, for one key head. The host has made sure that the units of a call with ascending offsets are below 2^32; of other
-    /// offsets they stay at 2^32 - 1.
+    /// Of some sequences, for one key head. The host has made sure that the units of a call whose offsets ascend are below 2^32.
     struct Count {
-        uint32_t units, blocks, most;  // most: units of one block
-        __device__ __forceinline__ void add(uint32_t u, uint32_t b, uint32_t m)
-        {
-            units += u, blocks += b, most = max(most, m);
-            if (units < u) units = ~0u;
-        }
+        uint32_t units, blocks, most;  // most: units of one block; ~0: offsets that descend
+        __device__ __forceinline__ void add(uint32_t u, uint32_t b, uint32_t m) { units += u, blocks += b, most = max(most, m); }
     };
     struct Shared {
         Count warp_sum[THREADS / 32], cost[THREADS];
@@ -184,8 +179,9 @@ struct Line {
             q = seq_at(p, s);
             const uint32_t blocks = blocks_of<ROWS>(p, q);
             many = blocks > 2;
+            if (blocks == 0 && paged::start_of(p.seqs, s + 1) < q.row0) mine.most = ~0u;
             if (many) sh.many[atomicAdd(&sh.n_many, 1u)] = tid;
-            else mine = count(p, q, blocks, 0, 1);
+            else if (blocks) mine = count(p, q, blocks, 0, 1);
         }
         __syncthreads();
         for (uint32_t i = warp; i < sh.n_many; i += THREADS / 32) {
@@ -237,7 +233,7 @@ struct Line {
                 all.add(t.units, t.blocks, t.most);
             }
         }
-        if ((uint64_t)all.units * p.cache.n_kv_heads >= 0xffffffffull) return false;  // offsets that are none
+        if (all.most == ~0u) return false;
         // The longest part: units cut evenly and an item's second part, or as many of the largest items as a part has items.
         const uint32_t items = all.blocks * p.cache.n_kv_heads, units = all.units * p.cache.n_kv_heads;
         whole = (items + p.parts - 1) / p.parts * (uint64_t)all.most <= units / p.parts + EXTRA;
