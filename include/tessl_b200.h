@@ -524,7 +524,14 @@ TESSL_API uint64_t tessl_attn_paged_workspace_bytes(TesslRuntime *rt, uint32_t t
  * rounded to bf16 for the product with v, after the sum over them was taken. An
  * infinity or NaN in v of a token reaches the rows that see it, in its column, a
  * score that is +infinity or NaN makes its row NaN; rows that do not see a token
- * are as if it were not there. A call of more than 2^32 units of 16 rows by 64 keys is refused. */
+ * are as if it were not there.
+ * Refused is a call of 2^32 units of work or more, where every sequence is taken to
+ * be as long as its row of the page table (the host does not see the lengths):
+ * n_kv_heads times blocks of rows (total_new * n_heads / n_kv_heads / R, and one for
+ * each sequence) times units of keys (max_pages * page_size / U, and one). R and U
+ * are 16 and 64, or, for calls of more than 32 rows of a key head and sequence on
+ * average, with q_starts, pages of a multiple of 8 tokens and a scale other than 0,
+ * 256 (128 for heads of more than 128) and 128. */
 TESSL_API int32_t tessl_attn_paged(TesslRuntime *rt, TesslBuf q, const TesslPagedKv *cache, const TesslPagedSeqs *seqs,
                                    TesslBuf out, TesslBuf workspace, uint32_t total_new, uint32_t n_heads,
                                    uint32_t q_stride, float scale, uint32_t causal, uint32_t window, char *err,

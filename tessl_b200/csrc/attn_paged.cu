@@ -47,6 +47,16 @@ uint32_t split_blocks(const TesslRuntime *rt, const TesslPagedKv &cache, const T
     return elems(seqs.num_seqs, cache.n_kv_heads) > (uint64_t)rt->sm_count ? 2 : 1;
 }
 
+/// Whether a call whose sequences are as long as their rows of the page table has more units than the kernels count, in 32 bits: what they
+/// count are the blocks of rows and the units of keys of the route that the call takes.
+bool too_much(const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t group, bool tiles)
+{
+    const double rows = tiles ? with_dim(cache.head_dim, [](auto dp) { return (double)attn::TileCfg<decltype(dp)::value>::ROWS; }) : attn::kSplitRows;
+    const double blocks = (double)elems(total_new, group) / rows + seqs.num_seqs;
+    const double most = (double)std::min<uint64_t>(elems(seqs.max_pages, cache.page_size), 0x7fffffffu) / (tiles ? attn::kTileKeys : attn::kSplitUnit) + 1;
+    return blocks * most * cache.n_kv_heads >= 4294967296.0;
+}
+
 uint64_t workspace_of(const TesslRuntime *rt, const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t group)
 {
     return with_dim(cache.head_dim, [&](auto dp) -> uint64_t {
@@ -152,9 +162,10 @@ Result attn_paged(TesslRuntime *rt, const TesslBuf &q, const TesslPagedKv &cache
     TESSL_TRY(require_aligned16(q, "attn_paged q"));
     TESSL_TRY(require_aligned16(out, "attn_paged out"));
     if (q_stride % 8 != 0) return fmt("%s: rows of q are %u apart, not a multiple of 8", what, q_stride);
-    // The kernels count 16 rows x 64 keys at a time, in 32 bits.
-    const double blocks = (double)elems(total_new, p.group.d) / 16 + seqs.num_seqs, most = (double)std::min<uint64_t>(p.seqs.capacity, 0x7fffffffu) / 64 + 1;
-    if (blocks * most * cache.n_kv_heads >= 4294967296.0) return fmt("%s: more rows and keys than one call counts", what);
+    // A scale of zero makes zeros of scores that a mask has set to -inf: the tile kernel masks before it scales.
+    p.scale_log2 = scale * 1.4426950408889634f;
+    const bool tiles = wants_tiles(cache, seqs, total_new, p.group.d) && p.scale_log2 != 0.0f;
+    if (too_much(cache, seqs, total_new, p.group.d, tiles)) return fmt("%s: more rows and keys than one call counts", what);
     const uint64_t need = workspace_of(rt, cache, seqs, total_new, p.group.d);
     if (workspace.nbytes < need) return fmt("%s: the workspace has %llu bytes, the call needs %llu", what, (unsigned long long)workspace.nbytes, (unsigned long long)need);
     TESSL_TRY(require_aligned16(workspace, "attn_paged workspace"));
@@ -168,10 +179,7 @@ Result attn_paged(TesslRuntime *rt, const TesslBuf &q, const TesslPagedKv &cache
     p.q_stride = q_stride;
     if (cache.num_pages == 0) p.cache.k = p.cache.v = static_cast<uint16_t *>(q.ptr);  // copies of no bytes still name an address
     p.causal = causal, p.window = window, p.status = rt->status_dev;
-    p.scale_log2 = scale * 1.4426950408889634f;
     p.mark = next_mark(rt);
-    // A scale of zero makes zeros of scores that a mask has set to -inf: the tile kernel masks before it scales.
-    const bool tiles = wants_tiles(cache, seqs, total_new, p.group.d) && p.scale_log2 != 0.0f;
     const bool two = split_blocks(rt, cache, seqs) == 2;
     return with_dim(cache.head_dim, [&](auto dp) {
         constexpr int DP = decltype(dp)::value;

@@ -1,0 +1,63 @@
+"""attn_paged: which sizes it takes, and the workspace that it asks for. No GPU: every call ends in a refusal, that of its workspace at the
+latest."""
+import pytest
+
+from tessl_b200 import nn
+from test_attn_paged_refusals import host_rt  # noqa: F401
+
+
+def sizes(n, pages_each, page=2048, kvh=8, dim=128, starts=True):
+    """A cache and sequences whose buffers are never touched, far apart and as large as they have to be."""
+    far = iter(range(1 << 48, 1 << 56, 1 << 46))
+    pages = 1 << 10
+    cache = nn.PagedKv(nn.GpuBuffer(next(far), 1 << 45), nn.GpuBuffer(next(far), 1 << 45), pages, page, kvh, dim)
+    return cache, nn.PagedSeqs(nn.GpuBuffer(next(far), 1 << 45), nn.GpuBuffer(next(far), 1 << 45),
+                               nn.GpuBuffer(next(far), 1 << 45) if starts else None, n, pages_each)
+
+
+def refusal(rt, cache, seqs, total, heads, work=16, **how):
+    """What a call with a workspace of 16 bytes is refused for."""
+    big = 1 << 45
+    with pytest.raises(nn.TesslError) as e:
+        nn.attn_paged(rt, nn.GpuBuffer(1 << 57, big), cache, seqs, nn.GpuBuffer(1 << 58, big), nn.GpuBuffer(1 << 59, work), total, heads,
+                      how.pop("scale", 0.125), **how)
+    return str(e.value)
+
+
+# sequences, new tokens, heads, pages of 2048 for each, head_dim
+TAKEN = [(1, 65536, 64, 512, 128),    # a prompt of 65536 with room for 2^20 tokens
+         (16, 65536, 64, 512, 256),
+         (4, 200000, 32, 1024, 64)]
+
+
+@pytest.mark.parametrize("n,total,heads,each,dim", TAKEN)
+def test_long_prompts_with_room_for_long_contexts_are_taken(host_rt, n, total, heads, each, dim):  # noqa: F811
+    cache, seqs = sizes(n, each, dim=dim)
+    assert "workspace has 16 bytes" in refusal(host_rt, cache, seqs, total, heads)
+
+
+@pytest.mark.parametrize("dim,rows", [(64, 256), (128, 256), (136, 128), (256, 128)])
+def test_a_call_is_refused_from_2_32_units_on(host_rt, dim, rows):  # noqa: F811
+    """A sequence, 8 query heads on each of 8 key heads: 8 (8 t / rows + 1) (c / 128 + 1) units of t new tokens and c tokens of room; with a
+    scale of 0 they are of 16 rows and 64 keys."""
+    each = 1024  # 2^21 tokens, 16385 units of 128 keys, 32769 of 64
+    cache, seqs = sizes(1, each, dim=dim)
+    for scale, r, units in ((0.125, rows, 16385), (-0.1, rows, 16385), (0.0, 16, 32769)):
+        total = -(-(2 ** 32 - 8 * units) * r // (64 * units))  # the first that is refused
+        assert "more rows and keys" in refusal(host_rt, cache, seqs, total, 64, scale=scale)
+        assert "workspace has 16 bytes" in refusal(host_rt, cache, seqs, total - 1, 64, scale=scale)
+
+
+def test_few_rows_are_counted_by_16_and_64(host_rt):  # noqa: F811
+    for page, starts in ((2048, False), (2044, True)):  # a token each, or pages that are no multiple of 8
+        n = 40000
+        units = -(-(1 << 21) // 64) + 1
+        each = -(-((units - 1) * 64) // page)
+        cache, seqs = sizes(n, each, page=page, starts=starts, kvh=1)
+        blocks = n * 64 / 16 + n
+        most = each * page / 64 + 1
+        assert blocks * most >= 2 ** 32
+        assert "more rows and keys" in refusal(host_rt, cache, seqs, n, 64)
+        few = int((2 ** 32 - 1) // (most * 5))
+        cache, seqs = sizes(few, each, page=page, starts=starts, kvh=1)
+        assert "workspace has 16 bytes" in refusal(host_rt, cache, seqs, few, 64)
