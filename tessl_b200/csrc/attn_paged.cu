@@ -31,12 +31,16 @@ auto with_dim(uint32_t head_dim, F f)
 /// swizzle's groups of eight rows.
 uint32_t box_of(uint32_t page_size, uint32_t most) { return std::min(page_size & (0u - page_size), most); }
 
+/// Whether the new tokens are given by offsets. A query of the workspace may come before there are any: without them a call has a new
+/// token for each sequence.
+bool with_starts(const TesslPagedSeqs &seqs, uint32_t total_new) { return seqs.q_starts.ptr || total_new != seqs.num_seqs; }
+
 /// Whether a call of these sizes goes to the tensor-core tiles: more than 32 rows for each key head of a sequence, on average. Eight
 /// sequences of up to 8000 keys, 32 heads of 128 on 8, with the kernel for few rows and with the tiles: 16 rows 56 and 60 us, 24 rows 66 and
 /// 60 us, 48 rows 83 and 61 us; one sequence: 32 rows 25 and 29 us, 64 rows 42 and 39 us; four sequences of wide heads: 32 rows 51 and 50 us.
 bool wants_tiles(const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t group)
 {
-    return seqs.q_starts.ptr && cache.num_pages > 0 && cache.page_size % 8 == 0 && elems(total_new, group) > 32ull * seqs.num_seqs;
+    return with_starts(seqs, total_new) && cache.num_pages > 0 && cache.page_size % 8 == 0 && elems(total_new, group) > 32ull * seqs.num_seqs;
 }
 
 /// Blocks of the split kernel on an SM: two, of half the warps each, where there are more items than SMs, so that one reads while the other
@@ -124,13 +128,20 @@ uint64_t next_mark(TesslRuntime *rt)
     return z ? z : 1;  // 0 is nobody's
 }
 
+Result heads_validate(const TesslPagedKv &cache, uint32_t total_new, uint32_t n_heads, const char *what)
+{
+    if (n_heads == 0 || n_heads % cache.n_kv_heads != 0)
+        return fmt("%s: n_heads %u is not a multiple of n_kv_heads %u", what, n_heads, cache.n_kv_heads);
+    TESSL_TRY(require_i32_extent(elems(total_new, n_heads), "attn_paged: total_new * n_heads"));
+    if (elems(n_heads, cache.head_dim) > 0xffffffffull) return fmt("%s: rows of %u heads are too long", what, n_heads);
+    return ok();
+}
+
 Result attn_params(const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t n_heads, const char *what, Params *p)
 {
     TESSL_TRY(paged::cache_validate(cache, what, &p->cache));
     TESSL_TRY(paged::seqs_validate(seqs, cache, total_new, what, &p->seqs));
-    if (n_heads == 0 || n_heads % cache.n_kv_heads != 0)
-        return fmt("%s: n_heads %u is not a multiple of n_kv_heads %u", what, n_heads, cache.n_kv_heads);
-    TESSL_TRY(require_i32_extent(elems(total_new, n_heads), "attn_paged: total_new * n_heads"));
+    TESSL_TRY(heads_validate(cache, total_new, n_heads, what));
     p->n_heads = n_heads, p->group = attn::Divisor::of(n_heads / cache.n_kv_heads), p->page = attn::Divisor::of(cache.page_size);
     return ok();
 }
@@ -141,10 +152,13 @@ namespace nn {
 
 uint64_t attn_paged_workspace_bytes(TesslRuntime *rt, uint32_t total_new, uint32_t n_heads, const TesslPagedKv &cache, const TesslPagedSeqs &seqs)
 {
-    if (cache.head_dim == 0 || cache.head_dim % 8 != 0 || cache.head_dim > 256 || cache.n_kv_heads == 0 || n_heads == 0 ||
-        n_heads % cache.n_kv_heads != 0 || elems(total_new, n_heads) > 0x7fffffffull)
+    const char *what = "attn_paged_workspace_bytes";
+    if (!paged::cache_sizes_validate(cache, what).empty() || !paged::seqs_sizes_validate(seqs, total_new, what).empty() ||
+        !heads_validate(cache, total_new, n_heads, what).empty())
         return 0;
-    return workspace_of(rt, cache, seqs, total_new, n_heads / cache.n_kv_heads);
+    const uint32_t group = n_heads / cache.n_kv_heads;
+    if (too_much(cache, seqs, total_new, group, wants_tiles(cache, seqs, total_new, group))) return 0;
+    return workspace_of(rt, cache, seqs, total_new, group);
 }
 
 Result attn_paged(TesslRuntime *rt, const TesslBuf &q, const TesslPagedKv &cache, const TesslPagedSeqs &seqs, const TesslBuf &out,

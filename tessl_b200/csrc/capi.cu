@@ -667,7 +667,11 @@ uint64_t tessl_attn_paged_workspace_bytes(TesslRuntime *rt, uint32_t total_new, 
                                           const TesslPagedSeqs *seqs)
 {
     if (!rt || !cache || !seqs) return 0;
-    return tessl::nn::attn_paged_workspace_bytes(rt, total_new, n_heads, *cache, *seqs);
+    try {
+        return tessl::nn::attn_paged_workspace_bytes(rt, total_new, n_heads, *cache, *seqs);
+    } catch (...) {
+        return 0;
+    }
 }
 
 int32_t tessl_attn_paged(TesslRuntime *rt, TesslBuf q, const TesslPagedKv *cache, const TesslPagedSeqs *seqs, TesslBuf out,

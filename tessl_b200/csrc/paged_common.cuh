@@ -58,16 +58,24 @@ __device__ __forceinline__ uint32_t seq_of_row(const Seqs &q, uint32_t row)
     return lo;
 }
 
-inline Result cache_validate(const TesslPagedKv &c, const char *what, Cache *out)
+/// A cache's sizes; its buffers may be missing yet.
+inline Result cache_sizes_validate(const TesslPagedKv &c, const char *what)
 {
     if (c.layout != TESSL_KV_TOKEN_MAJOR && c.layout != TESSL_KV_HEAD_MAJOR) return fmt("%s: unknown cache layout %u", what, c.layout);
     if (c.head_dim == 0 || c.head_dim % 8 != 0 || c.head_dim > 256)
         return fmt("%s: head_dim %u is not a multiple of 8 up to 256", what, c.head_dim);
     if (c.n_kv_heads == 0 || c.n_kv_heads > 65535) return fmt("%s: n_kv_heads %u is outside 1 .. 65535", what, c.n_kv_heads);
     if (c.page_size == 0) return fmt("%s: page_size must be non-zero", what);
-    const uint64_t row = elems(c.n_kv_heads, c.head_dim), page = row * c.page_size;  // row < 2^24
+    const uint64_t page = elems(c.n_kv_heads, c.head_dim) * c.page_size;  // a row < 2^24
     if (page > 0x7fffffffull) return fmt("%s: a page of %llu values is too large", what, (unsigned long long)page);
     if (c.num_pages > 0x7fffffffu) return fmt("%s: num_pages %u does not fit an int32 page id", what, c.num_pages);
+    return ok();
+}
+
+inline Result cache_validate(const TesslPagedKv &c, const char *what, Cache *out)
+{
+    TESSL_TRY(cache_sizes_validate(c, what));
+    const uint64_t row = elems(c.n_kv_heads, c.head_dim), page = row * c.page_size;
     const uint64_t need = page * c.num_pages;  // < 2^62
     TESSL_TRY(require(c.k, need, 2, What(what) + " cache k"));
     TESSL_TRY(require(c.v, need, 2, What(what) + " cache v"));
@@ -80,10 +88,16 @@ inline Result cache_validate(const TesslPagedKv &c, const char *what, Cache *out
     return ok();
 }
 
-inline Result seqs_validate(const TesslPagedSeqs &s, const TesslPagedKv &c, uint32_t total_new, const char *what, Seqs *out)
+inline Result seqs_sizes_validate(const TesslPagedSeqs &s, uint32_t total_new, const char *what)
 {
     if (s.num_seqs > 0x7fffffffu || total_new > 0x7fffffffu)
         return fmt("%s: %u sequences, %u new tokens: more than an int32 offset counts", what, s.num_seqs, total_new);
+    return ok();
+}
+
+inline Result seqs_validate(const TesslPagedSeqs &s, const TesslPagedKv &c, uint32_t total_new, const char *what, Seqs *out)
+{
+    TESSL_TRY(seqs_sizes_validate(s, total_new, what));
     TESSL_TRY(require(s.page_table, elems(s.num_seqs, s.max_pages), 4, What(what) + " page_table"));
     TESSL_TRY(require(s.kv_lens, s.num_seqs, 4, What(what) + " kv_lens"));
     if (s.q_starts.ptr) {

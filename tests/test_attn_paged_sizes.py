@@ -1,5 +1,7 @@
 """attn_paged: which sizes it takes, and the workspace that it asks for. No GPU: every call ends in a refusal, that of its workspace at the
 latest."""
+from dataclasses import replace
+
 import pytest
 
 from tessl_b200 import nn
@@ -61,3 +63,45 @@ def test_few_rows_are_counted_by_16_and_64(host_rt):  # noqa: F811
         few = int((2 ** 32 - 1) // (most * 5))
         cache, seqs = sizes(few, each, page=page, starts=starts, kvh=1)
         assert "workspace has 16 bytes" in refusal(host_rt, cache, seqs, few, 64)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(layout=2), "layout 2"), (dict(head_dim=0), "head_dim 0"), (dict(head_dim=60), "head_dim 60"), (dict(head_dim=264), "head_dim 264"),
+    (dict(n_kv_heads=0), "n_kv_heads 0"), (dict(n_kv_heads=65536), "n_kv_heads 65536"), (dict(page_size=0), "page_size"),
+    (dict(page_size=1 << 25), "too large"), (dict(num_pages=1 << 31), "page id"), (dict(n_kv_heads=3), "not a multiple"),
+])
+def test_the_workspace_of_a_cache_that_is_refused_is_none(host_rt, change, match):  # noqa: F811
+    cache, seqs = sizes(3, 4, page=16)
+    bad = replace(cache, **change)
+    heads = max(16, change.get("n_kv_heads", 0))
+    assert match in refusal(host_rt, bad, seqs, 3, heads)
+    assert nn.attn_paged_workspace_bytes(host_rt, 3, heads, bad, seqs) == 0
+
+
+def test_the_workspace_of_a_call_that_is_refused_is_none(host_rt):  # noqa: F811
+    cache, seqs = sizes(3, 4, page=16)
+    ask = lambda total, heads, c=cache, s=seqs: nn.attn_paged_workspace_bytes(host_rt, total, heads, c, s)
+    assert ask(3, 16) > 0
+    for heads in (0, 12, 1 << 30):
+        assert ask(3, heads) == 0 and refusal(host_rt, cache, seqs, 3, heads)
+    for total in (1 << 31, (1 << 32) - 1):
+        assert ask(total, 8) == 0 and "int32 offset" in refusal(host_rt, cache, seqs, total, 8)
+    assert ask(3, 8, s=replace(seqs, num_seqs=1 << 31)) == 0
+    # rows of 2^24 heads of 256 columns: 2^32 values
+    wide, one = sizes(1, 4, page=16, dim=256)
+    assert ask(1, 1 << 24, wide, one) == 0 and "too long" in refusal(host_rt, wide, one, 1, 1 << 24)
+    assert ask(1, (1 << 24) - 8, wide, one) > 0
+    # more units than are counted
+    long, s = sizes(1, 1024)
+    last = -(-(2 ** 32 - 8 * 16385) * 256 // (64 * 16385)) - 1
+    assert ask(last, 64, long, s) > 0 and ask(last + 1, 64, long, s) == 0
+    assert "more rows and keys" in refusal(host_rt, long, s, last + 1, 64)
+
+
+def test_a_workspace_can_be_asked_for_before_there_are_buffers(host_rt):  # noqa: F811
+    cache, seqs = sizes(3, 4, page=16)
+    none = nn.GpuBuffer(0, 0)
+    early = replace(seqs, page_table=none, kv_lens=none, q_starts=None)
+    for total in (200, 3):
+        want = nn.attn_paged_workspace_bytes(host_rt, total, 64, cache, seqs if total == 200 else replace(seqs, q_starts=None))
+        assert 0 < want == nn.attn_paged_workspace_bytes(host_rt, total, 64, replace(cache, k=none, v=none), early)
