@@ -510,9 +510,11 @@ TESSL_API int32_t tessl_kv_append_paged(TesslRuntime *rt, TesslBuf q, TesslBuf k
  * heads, the units of work counted below for a scale other than 0). Of the buffers
  * only q_starts is looked at: whether there are offsets. Without them, and with
  * other than one new token for each sequence, they are taken to come by the time of
- * the call. The contents need no preparation and mean nothing between calls. Calls
- * that may overlap on the GPU (graphs replayed on other streams) need workspaces of
- * their own. */
+ * the call. With offsets, the size is enough for every call over this cache with
+ * these heads of as many new tokens and sequences or fewer, with or without offsets:
+ * a host asks once, for its largest batch. The contents need no preparation and mean
+ * nothing between calls. Calls that may overlap on the GPU (graphs replayed on other
+ * streams) need workspaces of their own. */
 TESSL_API uint64_t tessl_attn_paged_workspace_bytes(TesslRuntime *rt, uint32_t total_new, uint32_t n_heads,
                                                     const TesslPagedKv *cache, const TesslPagedSeqs *seqs);
 

@@ -35,12 +35,18 @@ uint32_t box_of(uint32_t page_size, uint32_t most) { return std::min(page_size &
 /// token for each sequence.
 bool with_starts(const TesslPagedSeqs &seqs, uint32_t total_new) { return seqs.q_starts.ptr || total_new != seqs.num_seqs; }
 
+/// Whether a call of so many new tokens or fewer, of so many sequences or fewer, may go to the tensor-core tiles: all tokens may be of one.
+bool may_want_tiles(const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t group)
+{
+    return with_starts(seqs, total_new) && cache.num_pages > 0 && cache.page_size % 8 == 0 && elems(total_new, group) > 32;
+}
+
 /// Whether a call of these sizes goes to the tensor-core tiles: more than 32 rows for each key head of a sequence, on average. Eight
 /// sequences of up to 8000 keys, 32 heads of 128 on 8, with the kernel for few rows and with the tiles: 16 rows 56 and 60 us, 24 rows 66 and
 /// 60 us, 48 rows 83 and 61 us; one sequence: 32 rows 25 and 29 us, 64 rows 42 and 39 us; four sequences of wide heads: 32 rows 51 and 50 us.
 bool wants_tiles(const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t group)
 {
-    return with_starts(seqs, total_new) && cache.num_pages > 0 && cache.page_size % 8 == 0 && elems(total_new, group) > 32ull * seqs.num_seqs;
+    return may_want_tiles(cache, seqs, total_new, group) && elems(total_new, group) > 32ull * seqs.num_seqs;
 }
 
 /// Blocks of the split kernel on an SM: two, of half the warps each, where there are more items than SMs, so that one reads while the other
@@ -61,13 +67,13 @@ bool too_much(const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t to
     return blocks * most * cache.n_kv_heads >= 4294967296.0;
 }
 
-uint64_t workspace_of(const TesslRuntime *rt, const TesslPagedKv &cache, const TesslPagedSeqs &seqs, uint32_t total_new, uint32_t group)
+uint64_t workspace_of(const TesslRuntime *rt, const TesslPagedKv &cache, const TesslPagedSeqs &seqs, bool tiles)
 {
     return with_dim(cache.head_dim, [&](auto dp) -> uint64_t {
         constexpr int DP = decltype(dp)::value;
         const uint64_t few = attn::Part<attn::kSplitRows, DP>::bytes((uint64_t)rt->sm_count * split_blocks(rt, cache, seqs));
         const uint64_t many = attn::Part<attn::TileCfg<DP>::ROWS, DP>::bytes(rt->sm_count);
-        return wants_tiles(cache, seqs, total_new, group) ? std::max(few, many) : few;
+        return tiles ? std::max(few, many) : few;
     });
 }
 
@@ -158,7 +164,7 @@ uint64_t attn_paged_workspace_bytes(TesslRuntime *rt, uint32_t total_new, uint32
         return 0;
     const uint32_t group = n_heads / cache.n_kv_heads;
     if (too_much(cache, seqs, total_new, group, wants_tiles(cache, seqs, total_new, group))) return 0;
-    return workspace_of(rt, cache, seqs, total_new, group);
+    return workspace_of(rt, cache, seqs, may_want_tiles(cache, seqs, total_new, group));
 }
 
 Result attn_paged(TesslRuntime *rt, const TesslBuf &q, const TesslPagedKv &cache, const TesslPagedSeqs &seqs, const TesslBuf &out,
@@ -180,7 +186,7 @@ Result attn_paged(TesslRuntime *rt, const TesslBuf &q, const TesslPagedKv &cache
     p.scale_log2 = scale * 1.4426950408889634f;
     const bool tiles = wants_tiles(cache, seqs, total_new, p.group.d) && p.scale_log2 != 0.0f;
     if (too_much(cache, seqs, total_new, p.group.d, tiles)) return fmt("%s: more rows and keys than one call counts", what);
-    const uint64_t need = workspace_of(rt, cache, seqs, total_new, p.group.d);
+    const uint64_t need = workspace_of(rt, cache, seqs, tiles);
     if (workspace.nbytes < need) return fmt("%s: the workspace has %llu bytes, the call needs %llu", what, (unsigned long long)workspace.nbytes, (unsigned long long)need);
     TESSL_TRY(require_aligned16(workspace, "attn_paged workspace"));
     if (!workspace.ptr) return fmt("%s: null workspace", what);

@@ -498,7 +498,7 @@ def kv_append_paged(rt: Runtime, q: Optional[GpuBuffer], k: GpuBuffer, v: GpuBuf
 
 def attn_paged_workspace_bytes(rt: Runtime, total_new: int, n_heads: int, cache: PagedKv, seqs: PagedSeqs) -> int:
     """Bytes of workspace that `attn_paged` wants for a call of these sizes; 0 for sizes that it refuses (buffers are not looked at but
-    for whether there are offsets)."""
+    for whether there are offsets). With offsets it is enough for every smaller batch too, of fewer new tokens, sequences or both."""
     return int(capi.load().tessl_attn_paged_workspace_bytes(rt.handle, total_new, n_heads, C.byref(cache.c()), C.byref(seqs.c())))
 
 

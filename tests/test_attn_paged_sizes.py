@@ -1,5 +1,6 @@
 """attn_paged: which sizes it takes, and the workspace that it asks for. No GPU: every call ends in a refusal, that of its workspace at the
 latest."""
+import re
 from dataclasses import replace
 
 import pytest
@@ -105,3 +106,26 @@ def test_a_workspace_can_be_asked_for_before_there_are_buffers(host_rt):  # noqa
     for total in (200, 3):
         want = nn.attn_paged_workspace_bytes(host_rt, total, 64, cache, seqs if total == 200 else replace(seqs, q_starts=None))
         assert 0 < want == nn.attn_paged_workspace_bytes(host_rt, total, 64, replace(cache, k=none, v=none), early)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+@pytest.mark.parametrize("kvh,heads", [(8, 32), (1, 16), (4, 4), (2, 80)])
+def test_the_workspace_of_a_batch_serves_every_smaller_one(host_rt, dim, kvh, heads):  # noqa: F811
+    """What a call needs, by its refusal of 16 bytes, against what the query says of larger batches."""
+    tokens, counts = (1, 2, 3, 9, 33, 64, 65, 300, 4096), (1, 2, 19, 37, 64, 75, 300)
+    need, asked = {}, {}
+    for n in counts:
+        for total in tokens:
+            for starts in (True, False) if total == n else (True,):
+                cache, seqs = sizes(n, 4, page=16, kvh=kvh, dim=dim, starts=starts)
+                need[total, n, starts] = int(re.search(r"needs (\d+)", refusal(host_rt, cache, seqs, total, heads)).group(1))
+                if starts:
+                    asked[total, n] = nn.attn_paged_workspace_bytes(host_rt, total, heads, cache, seqs)
+    for (t, n, _), least in need.items():
+        for (total, most), size in asked.items():
+            if t <= total and n <= most:
+                assert size >= least > 0, ((t, n), (total, most))
+    for (t, n, starts), least in need.items():  # a token each, without offsets: no more than such calls want
+        if not starts:
+            cache, seqs = sizes(n, 4, page=16, kvh=kvh, dim=dim, starts=False)
+            assert nn.attn_paged_workspace_bytes(host_rt, t, heads, cache, seqs) == least
