@@ -98,14 +98,16 @@ __device__ __forceinline__ void store_run(void *dst, size_t at, const float (&v)
 }
 
 /// factor * (cos, sin) of 2 pi angle / 2^32. Polynomials with the least relative error for |x| <= 1/4 (Remez, the leading coefficients
-/// held at their f32 values while the others are fitted): sin(pi x) = x (pi + P(x^2)) to 3.4e-9, cos(pi x) = Q(x^2) to 6.4e-10 with the
-/// coefficients as they stand here. P's constant holds what f32 leaves out of pi. With the rounding in f32 both are within
-/// 2.5 * 2^-24 of themselves (1.82 and 1.59 over 5 million angles); pi in one f32 took the sine to 2.9.
+/// held at their f32 values while the others are fitted): sin(pi x) = pi x + (d x + x^3 P(x^2)) to 3.4e-9, cos(pi x) = Q(x^2) to 6.4e-10 with the
+/// coefficients as they stand here. d is what f32 leaves out of pi. With the rounding in f32 both are within
+/// 2.5 * 2^-24 of themselves (1.82 and 1.59 over 5 million angles); pi in one f32 took the sine to 2.9. (With d in P's place, the compiler
+/// ordered the loads of the kernel below otherwise: 8192 tokens x 32 heads of 128 in 29.4 us instead of 25.9.)
 __device__ __forceinline__ float2 turn_of(uint32_t angle, float factor)
 {
     const uint32_t quadrant = (angle + 0x20000000u) >> 30;
     const float x = (float)(int32_t)(angle - (quadrant << 30)) * 0x1p-31f, t = x * x;
-    const float s = fmaf(x, 3.1415927410f, x * fmaf(fmaf(fmaf(-0.5890811086f, t, 2.5497686863f), t, -5.1677079201f), t, -9.571968462e-8f));
+    const float odd = x * t * fmaf(fmaf(-0.5890811086f, t, 2.5497686863f), t, -5.1677079201f);
+    const float s = fmaf(x, 3.1415927410f, fmaf(x, -9.571968462e-8f, odd));
     const float c = fmaf(fmaf(fmaf(fmaf(0.2289538831f, t, -1.3347475529f), t, 4.0586962700f), t, -4.9348020554f), t, 1.0f);
     const float sf = quadrant & 2u ? -factor : factor, cf = (quadrant + 1) & 2u ? -factor : factor;
     return quadrant & 1u ? make_float2(cf * s, sf * c) : make_float2(cf * c, sf * s);

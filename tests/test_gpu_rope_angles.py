@@ -25,8 +25,8 @@ def test_angles(rt, kind, dim, interleaved):
     """Pairs (1, 0) turned: what comes out is the cosine and the sine alone.
 
     Relative error, u = 2^-24, x half a turn's fraction of at most 1/4: the angle to f32 u, which counts as pi x cot(pi x) <= 1 (sine) or
-    pi x tan(pi x) <= 0.79 (cosine). Sine: beside pi, the polynomial is 0.11 of it at most; its argument's square, its last
-    two roundings and their product with x 4 * 0.11 u; the polynomial itself 0.06 u; the last sum u. At x = 1/4, 0.79 + 0.44 + 0.06 + 1;
+    pi x tan(pi x) <= 0.79 (cosine). Sine: beside pi, the polynomial is 0.11 of it at most; the square of x, its
+    product with x, the last rounding of the polynomial and its product 4 * 0.11 u; the polynomial itself 0.06 u; the last sum u. At x = 1/4, 0.79 + 0.44 + 0.06 + 1;
     towards 0, where the polynomial vanishes, 1 + 1. Cosine: 1 - cos is 0.42 of it at most, off by the square's rounding and the last
     sum's before the end, 2 * 0.42 u, and 0.1 of that by the sums before; the polynomial 0.01 u; the last sum 0.71 u (2^-25 of a value
     from 0.70 on): 0.79 + 0.92 + 0.01 + 0.71. Both below 2.5 u."""
