@@ -530,7 +530,14 @@ TESSL_API uint64_t tessl_attn_paged_workspace_bytes(TesslRuntime *rt, uint32_t t
  * rounded to bf16 for the product with v, after the sum over them was taken. An
  * infinity or NaN in v of a token reaches the rows that see it, in its column, a
  * score that is +infinity or NaN makes its row NaN; rows that do not see a token
- * are as if it were not there.
+ * are as if it were not there. Products of v with weights of up to 2^8 are added up
+ * in f32 and divided at the end: values that add up to 2^120 over a row's keys may
+ * make it infinite.
+ * One kernel for few rows or one for many (more than 32 of a key head and sequence)
+ * serves a whole call, by the mean over its sequences, those without new tokens
+ * counted. Every batch is served rightly; where a chunk of some hundred tokens
+ * stands beside many single ones, two calls (over parts of q, out, the table and
+ * the lengths; one workspace) are up to four times as fast as one.
  * Refused is a call of 2^32 units of work or more, where every sequence is taken to
  * be as long as its row of the page table (the host does not see the lengths):
  * n_kv_heads times blocks of rows (total_new * n_heads / n_kv_heads / R, and one for

@@ -13,8 +13,8 @@
 // The weights p of a step are rounded to bf16 for the product with V: relative 2^-8 at most, each its own way, against the 2^-8 of
 // the output's own rounding; their sum is taken in f32 before that.
 //
-// Bound by memory: a step of 16 keys is 64 D bytes and D / 2 MMAs of 16 x 8 x 16. 32 heads of 128 on 8, a token over 130001 keys: 101 us,
-// 5.3 TB/s; 64 tokens over up to 12000 keys each: 273 us, 5.9 TB/s, of 6.6 that a copy reaches. Over a few hundred keys the time is
+// Bound by memory: a step of 16 keys is 64 D bytes and D / 4 MMAs of 16 x 8 x 16. 32 heads of 128 on 8, a token over 130001 keys: 102 us,
+// 5.2 TB/s; 64 tokens over up to 12000 keys each: 287 us, 5.6 TB/s, of 6.6 that a copy reaches (call behind call 273 us). Over a few hundred keys the time is
 // latency: 2 us to the first request (lengths, then page ids), 1 us to the first tile, 0.7 us for the warps to meet, 4 us to join parts.
 #pragma once
 #include "attn_paged_common.cuh"

@@ -18,7 +18,8 @@
 // Rounding of the weights: see attn_paged_split.cuh.
 //
 // Bound by the chain scores, softmax, weights, product of a step, of which a row tile has two under way: 1024 tokens over 33024 keys, 32
-// heads of 128 on 8, take 520 us (1048 TFLOP/s, of 1668 for a library product), a prompt of 4096 with 16 heads of 256 on 4 216 us (635
+// heads of 128 on 8, take 615 us call behind call (888 TFLOP/s, of 1382 for a library product that runs as long: both at the power cap, this
+// at 1570 MHz) and 529 us in the first calls after a pause (1030 of 1668, at 1965 MHz); a prompt of 4096 with 16 heads of 256 on 4 215 us (639
 // TFLOP/s): wide heads have one row tile, with two threads for a row that wait for each other's maxima.
 //
 // Roles: eight warps softmax, Q and the results, one warp TMA, a warp for each row tile MMA issue. Every wait is bounded; on a
