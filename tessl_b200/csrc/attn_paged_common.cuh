@@ -16,6 +16,8 @@
 namespace tessl {
 namespace attn {
 
+using paged::bf16_pair;
+
 /// Division by a number that is the same for a whole launch, exact for every 32-bit dividend: the multiplication by a rounded-up
 /// reciprocal of Granlund and Montgomery. (The compiler's division is some thirty instructions, and what a block does once it runs from
 /// a cold instruction cache.)
@@ -329,12 +331,6 @@ __device__ __forceinline__ float exp2_fast(float x)
 {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi)
-{
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
 

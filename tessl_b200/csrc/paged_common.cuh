@@ -7,6 +7,14 @@
 namespace tessl {
 namespace paged {
 
+/// Two f32 -> a bf16 pair, to nearest even.
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
 /// The cache as the kernels address it; strides in elements.
 struct Cache {
     uint16_t *k, *v;

@@ -20,6 +20,8 @@
 namespace tessl {
 namespace {
 
+using paged::bf16_pair;
+
 constexpr uint32_t kThreads = 32;  // a warp: blocks of four ended later, 8192 tokens x 32 heads of 128 in 31.1 us instead of 26.9
 constexpr uint32_t kMaxPairs = 128;  // of a head of 256
 
@@ -69,14 +71,6 @@ struct Run {
         }
     }
 };
-
-/// Two f32 -> a bf16 pair, to nearest even.
-__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi)
-{
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 
 template <bool OUT16, int VEC>
 __device__ __forceinline__ void store_run(void *dst, size_t at, const float (&v)[VEC])
