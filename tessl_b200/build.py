@@ -59,7 +59,7 @@ def build_library(verbose_ptxas: bool = False) -> None:
     LIB.parent.mkdir(parents=True, exist_ok=True)
     host_cxx = "/usr/bin/g++" if Path("/usr/bin/g++").exists() else None
     cmd = [nvcc_path(), "-std=c++17", "-O3", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
-           "-shared", "-Xcompiler", "-fPIC,-fvisibility=hidden", "--expt-relaxed-constexpr",
+           "--threads", "0", "-shared", "-Xcompiler", "-fPIC,-fvisibility=hidden", "--expt-relaxed-constexpr",
            "-Xlinker", "--exclude-libs,ALL"]
     if host_cxx:
         cmd += ["-ccbin", host_cxx]
